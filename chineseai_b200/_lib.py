@@ -30,6 +30,30 @@ class FWeights(C.Structure):
         "ft_weight", "ft_bias", "l1_weight", "l1_bias", "l2_weight", "l2_bias", "l3_weight", "l3_bias")]
 
 
+class LogitRules(C.Structure):
+    """cnnue_logit_rules."""
+    _fields_ = [("history", c_void_p), ("history_stride", c_i64), ("history_len", c_i64), ("history_bytes", c_int),
+                ("lengths", c_void_p), ("prompt_lengths", c_void_p), ("repetition", c_void_p),
+                ("frequency", c_void_p), ("presence", c_void_p), ("bias_tokens", c_void_p),
+                ("bias_tokens_stride", c_i64), ("bias_values", c_void_p), ("bias_values_stride", c_i64),
+                ("bias_count", c_i64), ("mask", c_void_p), ("mask_stride", c_i64), ("mask_rows", c_i64),
+                ("mask_index", c_void_p)]
+
+
+class LossTargets(C.Structure):
+    """cnnue_loss_targets."""
+    _fields_ = [("dense", c_void_p), ("dense_stride", c_i64), ("dense_type", c_int), ("index", c_void_p),
+                ("index_stride", c_i64), ("index_bytes", c_int), ("prob", c_void_p), ("prob_stride", c_i64),
+                ("count", c_i64), ("mask", c_void_p), ("mask_stride", c_i64), ("mask_rows", c_i64),
+                ("mask_index", c_void_p), ("weights", c_void_p)]
+
+
+class AdamwTensor(C.Structure):
+    """cnnue_adamw_tensor."""
+    _fields_ = [(n, c_void_p) for n in ("param", "grad", "m", "v", "m_scale", "v_scale", "copy")] + \
+        [("n", c_i64)] + [(n, C.c_int16) for n in ("param_type", "grad_type", "copy_type", "flags")]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "cnnue_status_string": (C.c_char_p, [c_int]),
@@ -73,6 +97,12 @@ SIGNATURES = {
                             c_i64, P]),
     "cnnue_adamw_device": (c_int, [P, P, P, P, c_i64, P, P]),
     "cnnue_adamw_device_scaled": (c_int, [P, P, P, P, c_i64, P, C.c_float, P, c_int, P]),
+    "cnnue_adamw_multi": (c_int, [P, c_i64, c_int] + [C.c_double] * 5 + [c_i64, C.c_float, P, c_int, P]),
+    "cnnue_adamw_multi_device": (c_int, [P, c_i64, c_int, P, C.c_float, P, c_int, P]),
+    "cnnue_logits_process": (c_int, [P, c_i64, c_int, P, c_i64, c_int, c_i64, c_i64, P, P, P]),
+    "cnnue_policy_loss_fwd": (c_int, [P, c_i64, c_int, c_i64, c_i64, P, P, P, P, P]),
+    "cnnue_policy_loss_bwd": (c_int, [P, c_i64, c_int, c_i64, c_i64, P, P, P, P, c_i64, P, P]),
+    "cnnue_policy_loss_grad": (c_int, [P, c_i64, c_int, c_i64, c_i64, P, P, P, c_i64, P, P]),
     "cnnue_t_param_count": (c_size, []),
     "cnnue_t_workspace_bytes": (c_size, [c_i64, c_u32]),
     "cnnue_t_make_shadow": (c_int, [P, P, P]),
@@ -119,6 +149,7 @@ SIGNATURES = {
     "cnnue_azt_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64, c_i64]),
     "cnnue_azt_step": (c_int, [c_void_p, P, P, c_i64, P, c_i64, P, C.c_float, C.c_float, P, P, P, c_size, P, P]),
     "cnnue_az_legal_moves": (c_int, [P, c_int, P, c_int, C.POINTER(c_int)]),
+    "cnnue_az_legal_mask": (c_int, [P, P, c_i64, P, c_int]),
     "cnnue_mcts_default_limits": (None, [c_void_p]),
     "cnnue_mcts_create": (c_int, [c_void_p, c_void_p, c_int, C.POINTER(c_void_p)]),
     "cnnue_mcts_destroy": (c_int, [c_void_p]),

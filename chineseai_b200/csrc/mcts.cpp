@@ -1054,6 +1054,54 @@ int cnnue_az_legal_moves(const int8_t* board, int side, uint8_t* moves, int capa
   return CNNUE_OK;
 }
 
+int cnnue_az_legal_mask(const int8_t* boards, const uint8_t* sides, int64_t n, uint32_t* mask, int n_threads) {
+  if (n < 0 || (n > 0 && (!boards || !sides || !mask)))
+    return set_error(CNNUE_ERR_INVALID_ARG, "null boards, sides or mask, or negative n");
+  for (int64_t i = 0; i < n; ++i) {
+    if (sides[i] > 1) return set_error(CNNUE_ERR_INVALID_ARG, "sides[%lld] = %d", (long long)i, sides[i]);
+    for (int sq = 0; sq < kSq; ++sq)
+      if (boards[i * kSq + sq] < -7 || boards[i * kSq + sq] > 7)
+        return set_error(CNNUE_ERR_INVALID_ARG, "board %lld: [%d] = %d", (long long)i, sq, boards[i * kSq + sq]);
+  }
+  try {
+    std::vector<uint16_t> dense((size_t)kSq * kSq);
+    if (int st = cnnue_az_dense_moves(nullptr, dense.data())) return st;
+    std::atomic<int64_t> next{0};
+    std::atomic<bool> failed{false};
+    auto work = [&] {
+      try {
+        std::vector<Move> pseudo, legal;
+        for (int64_t i = next++; i < n; i = next++) {
+          uint32_t* words = mask + i * CNNUE_AZ_MASK_WORDS;
+          std::fill(words, words + CNNUE_AZ_MASK_WORDS, 0u);
+          legal_moves(boards + i * kSq, sides[i], pseudo, legal);
+          for (const Move& m : legal) {
+            const int from = sides[i] ? 89 - m.from : m.from, to = sides[i] ? 89 - m.to : m.to;
+            const uint16_t d = dense[(size_t)from * kSq + to];
+            if (d < CNNUE_AZ_DENSE_MOVES) words[d >> 5] |= 1u << (d & 31);
+          }
+        }
+      } catch (...) {
+        failed = true;
+      }
+    };
+    // threads pay from some hundred positions on (a position takes about 2 us)
+    int64_t t = n_threads > 0 ? n_threads : std::min<unsigned>(std::max(1u, std::thread::hardware_concurrency()), 16u);
+    t = std::min<int64_t>(t, n / 64);
+    std::vector<std::thread> pool;
+    try {
+      for (int64_t i = 1; i < t; ++i) pool.emplace_back(work);
+    } catch (...) {  // fewer threads than asked for
+    }
+    work();
+    for (std::thread& th : pool) th.join();
+    if (failed) return set_error(CNNUE_ERR_INTERNAL, "legal moves: out of host memory");
+  } catch (...) {
+    return set_error(CNNUE_ERR_INTERNAL, "legal moves: out of host memory");
+  }
+  return CNNUE_OK;
+}
+
 int cnnue_mcts_create(const cnnue_az_model* model, const cnnue_az_weights* weights, int n_threads, cnnue_mcts** out) {
   if (!model || !weights || !out) return set_error(CNNUE_ERR_INVALID_ARG, "null model, weights or out");
   cnnue_mcts* s = new (std::nothrow) cnnue_mcts();

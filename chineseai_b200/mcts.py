@@ -16,6 +16,9 @@ import numpy as np
 from ._lib import check, lib
 
 
+MASK_WORDS = 66  # ceil(2086 dense moves / 32)
+
+
 class Limits(C.Structure):
     """AzSearchLimits (src/az/alphazero.rs:22-66) less seed and root noise."""
     _fields_ = [("simulations", C.c_int64)] + \
@@ -41,6 +44,20 @@ def legal_moves(board: np.ndarray, side: int) -> np.ndarray:
     n = C.c_int()
     check(lib().cnnue_az_legal_moves(b.ctypes.data, side, out.ctypes.data, 128, C.byref(n)), "cnnue_az_legal_moves")
     return out[:n.value].copy()
+
+
+def legal_mask(boards: np.ndarray, sides: np.ndarray, n_threads: int = 0) -> np.ndarray:
+    """The legal moves of each position as packed masks over the dense move
+    space (canonical moves of the side to move): int32 [n][66], the mask words
+    of logits.process_logits and logits.policy_loss."""
+    b = np.ascontiguousarray(boards, np.int8).reshape(-1, 90)
+    s = np.ascontiguousarray(sides, np.uint8).reshape(-1)
+    if len(s) != len(b):
+        raise ValueError(f"{len(b)} boards and {len(s)} sides")
+    out = np.zeros((len(b), MASK_WORDS), np.int32)
+    check(lib().cnnue_az_legal_mask(b.ctypes.data, s.ctypes.data, len(b), out.ctypes.data, n_threads),
+          "cnnue_az_legal_mask")
+    return out
 
 
 def perft(board: np.ndarray, side: int, depth: int) -> int:

@@ -369,6 +369,122 @@ int cnnue_policy_table_bwd(const int64_t* d_indices, const float* d_grad_out, in
                            int terms, int64_t table_len, float* d_grad_table, void* d_workspace,
                            size_t workspace_bytes, void* stream);
 
+/* ---- logits: penalties, biases, masks; the masked policy loss ------------
+ * Rows of logits [n_rows][vocab] over any token space: the 2086 dense moves
+ * (cnnue_az_dense_moves), the 8100 from-to pairs, or a vocabulary.  Elements
+ * are fp32, bf16 or fp16; a row is contiguous, rows are `stride` elements
+ * apart (0 = one row for all, inputs only); a row may start at any element.
+ * No counterpart among the reference's GPU code: its search masks by listing
+ * the legal moves (src/az/alphazero.rs:959-1081) and its trainer adds -1e9
+ * (policy_mask, src/az/dataloader.rs:113-336; src/az/train_gpu_candle.rs:
+ * 221-305).
+ *
+ * A packed mask row is uint32 [ceil(vocab / 32)]: bit j of word w allows token
+ * 32 w + j (1 = allowed); bits past the vocabulary are ignored.  Row r of the
+ * logits uses mask row d_mask_index[r] (negative = everything is allowed) or,
+ * without an index, row r (mask_rows == n_rows) or row 0 (mask_rows == 1).
+ * An index past the last mask row sets CNNUE_STATUS_BAD_INDEX and the row
+ * allows nothing.  d_status is a device word the caller zeroes and reads
+ * (cnnue_read_status); the calls only enqueue work, allocate nothing and may
+ * be captured in a CUDA graph. */
+#define CNNUE_F32 0
+#define CNNUE_BF16 1
+#define CNNUE_F16 2
+
+/* The packed masks of the legal moves of n positions over the dense move
+ * space, as the side to move sees it (canonical moves, the space of the
+ * policy logits): boards int8 [n][90], sides uint8 [n], mask uint32
+ * [n][CNNUE_AZ_MASK_WORDS] (host buffers), on n_threads host threads (<= 0:
+ * up to 16).  Replaces the legal-move list of AzTree::expand
+ * (src/az/alphazero.rs:959-1081) for callers that mask whole rows. */
+#define CNNUE_AZ_MASK_WORDS 66 /* ceil(2086 / 32) */
+int cnnue_az_legal_mask(const int8_t* boards, const uint8_t* sides, int64_t n, uint32_t* mask, int n_threads);
+
+/* What cnnue_logits_process applies to a row, in this order; every part may
+ * be absent (null):
+ *   penalties: history [n_rows][history_len] tokens (history_bytes 4 or 8:
+ *     int32 or int64; negative = padding), of which the first lengths[r]
+ *     count (null: all) and of those the first prompt_lengths[r] are the
+ *     prompt (null: none).  A token that occurs: x = x > 0 ? x / repetition[r]
+ *     : x * repetition[r].  With c > 0 occurrences after the prompt: x = x -
+ *     frequency[r] * c, then x = x - presence[r].
+ *   biases: bias_tokens int32 and bias_values fp32 [n_rows][bias_count]
+ *     (negative token = no entry): x = x + value, repeated tokens in list
+ *     order.
+ *   mask: tokens that are not allowed become -inf, whatever their logit (a
+ *     NaN or an infinity there is not read).
+ * A token >= vocab sets CNNUE_STATUS_BAD_INDEX and is skipped; lengths[r]
+ * outside [0, history_len] sets CNNUE_STATUS_BAD_OFFSETS and is clamped. */
+typedef struct cnnue_logit_rules {
+  const void* history;
+  int64_t history_stride;
+  int64_t history_len;
+  int history_bytes;
+  const int32_t* lengths;         /* [n_rows] */
+  const int32_t* prompt_lengths;  /* [n_rows] */
+  const float* repetition;        /* [n_rows] */
+  const float* frequency;         /* [n_rows] */
+  const float* presence;          /* [n_rows] */
+  const int32_t* bias_tokens;
+  int64_t bias_tokens_stride;
+  const float* bias_values;
+  int64_t bias_values_stride;
+  int64_t bias_count;
+  const uint32_t* mask;
+  int64_t mask_stride;            /* words */
+  int64_t mask_rows;
+  const int32_t* mask_index;      /* [n_rows] */
+} cnnue_logit_rules;
+/* out has the logits' type or fp32; it may be the logits themselves (same
+ * pointer, type and stride) but may not overlap them otherwise.  Each step
+ * is one IEEE fp32 operation, the result is rounded once. */
+int cnnue_logits_process(const void* d_logits, int64_t logits_stride, int logits_type, void* d_out, int64_t out_stride,
+                         int out_type, int64_t n_rows, int64_t vocab, const cnnue_logit_rules* rules,
+                         uint32_t* d_status, void* stream);
+
+/* Masked softmax cross entropy.  Over the allowed tokens A of a row: M = max
+ * z, S = sum exp(z - M), T = sum t, loss = w (T log S + sum t (M - z)) and
+ * dloss/dz = w (T exp(z - M) / S - t), 0 outside A.  Targets t: either dense
+ * [n_rows][vocab] (fp32, bf16 or fp16) or lists of `count` tokens per row
+ * (index_bytes 4 or 8: int32 or int64; negative = no entry) with their
+ * probabilities (null: 1 each; count = 1 without probabilities = labels);
+ * repeated tokens add up in list order.  Targets on tokens that are not
+ * allowed are dropped.  A row of which nothing is left (no allowed logit
+ * above -inf) has loss 0 and gradient 0; so has a row of weight 0, which is
+ * not read.  A NaN at an allowed token makes the row's loss and gradient NaN;
+ * elsewhere it is not read.  A listed token >= vocab sets
+ * CNNUE_STATUS_BAD_INDEX and is skipped.  Takes the role of the policy part
+ * of compute_batch_loss (src/az/train_gpu_candle.rs:221-305). */
+typedef struct cnnue_loss_targets {
+  const void* dense;
+  int64_t dense_stride;
+  int dense_type;
+  const void* index;
+  int64_t index_stride;
+  int index_bytes;
+  const float* prob;
+  int64_t prob_stride;
+  int64_t count;
+  const uint32_t* mask;
+  int64_t mask_stride;
+  int64_t mask_rows;
+  const int32_t* mask_index; /* [n_rows] */
+  const float* weights;      /* [n_rows] or null (1) */
+} cnnue_loss_targets;
+/* Loss [n_rows], and per row M, S, T in d_stats [n_rows][3] for the backward
+ * pass; the gradient (logits' type) times the upstream gradient d_upstream
+ * [n_rows] (null: 1). */
+int cnnue_policy_loss_fwd(const void* d_logits, int64_t logits_stride, int logits_type, int64_t n_rows, int64_t vocab,
+                          const cnnue_loss_targets* targets, float* d_loss, float* d_stats, uint32_t* d_status,
+                          void* stream);
+int cnnue_policy_loss_bwd(const void* d_logits, int64_t logits_stride, int logits_type, int64_t n_rows, int64_t vocab,
+                          const cnnue_loss_targets* targets, const float* d_stats, const float* d_upstream, void* d_grad,
+                          int64_t grad_stride, uint32_t* d_status, void* stream);
+/* Loss and gradient (upstream 1) in one pass over the logits. */
+int cnnue_policy_loss_grad(const void* d_logits, int64_t logits_stride, int logits_type, int64_t n_rows, int64_t vocab,
+                           const cnnue_loss_targets* targets, float* d_loss, void* d_grad, int64_t grad_stride,
+                           uint32_t* d_status, void* stream);
+
 /* ---- training step (data parallel), HalfKA network --------------------- */
 /* One rank's step of the fp32-master / bf16-activation form of the quantised
  * network: FT 11340x1024 (bf16 shadow gathered, fp32 sums), pairwise product
@@ -452,7 +568,8 @@ typedef struct cnnue_adamw_state {
   double lr, beta1, beta2, eps, weight_decay;
   int64_t step;        /* steps taken; 0 before the first */
   float scalars[9];    /* written by the device: this step's fp32 factors */
-  float pad[3];        /* pad[0]: 1 when the last device step was skipped */
+  float pad[3];        /* pad[0]: 1 when the last device step was skipped;
+                          pad[1]: sqrt(1/(1-b2^t)) of the last step taken */
 } cnnue_adamw_state;
 int cnnue_adamw_device(float* d_params, float* d_m, float* d_v, const float* d_grads, int64_t n,
                        cnnue_adamw_state* d_state, void* stream);
@@ -464,6 +581,51 @@ int cnnue_adamw_device(float* d_params, float* d_m, float* d_v, const float* d_g
 int cnnue_adamw_device_scaled(float* d_params, float* d_m, float* d_v, const float* d_grads, int64_t n,
                               cnnue_adamw_state* d_state, float grad_scale, const float* d_skip, int n_skip,
                               void* stream);
+
+/* AdamW over many tensors at once, with 32-bit or 8-bit states.
+ * params and grads are fp32, bf16 or fp16 (CNNUE_F32 / CNNUE_BF16 /
+ * CNNUE_F16), each tensor contiguous.  state_bits 32: m and v fp32 [n], and
+ * the arithmetic of cnnue_adamw, operation for operation, on the fp32 value of
+ * the parameter (a 16-bit parameter is rounded once).  state_bits 8: blocks of
+ * 256 elements; m and u = sqrt(v) as e4m3 values [n] times one fp32 scale per
+ * block ([ceil(n / 256)]):
+ *   m = cm * sm, u = cu * su, v = u * u;  m' and v' as above;  u' = sqrt(v')
+ *   p' = p*(1 - lr*wd) - ((m' / (1-b1^t)) / (u' * sqrt(1/(1-b2^t)) + eps)) * lr
+ *   scale = max|x| * (1/448) (0 when that is below 2^-126), code = e4m3(x *
+ *   (448 / max|x|)) rounded to nearest even, u' > 0 never below 2^-9 of the
+ *   scale (a second moment above zero stays above zero)
+ * in fp32; the update uses m' and u' before they are rounded to 8 bits.  A
+ * NaN or infinity in a block's m' (u') makes the scale and the codes of that
+ * block's m (u) non-finite.
+ * copy (optional): the updated parameter rounded to copy_type (bf16 or fp16),
+ * e.g. the 16-bit weights of the next forward.  Tensors of n = 0 are allowed;
+ * no two tensors may overlap. */
+#define CNNUE_ADAMW_BLOCK 256
+#define CNNUE_ADAMW_NO_DECAY 1 /* flags: no weight decay for this tensor */
+typedef struct cnnue_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* m;
+  void* v;            /* 8 bits: the codes of u */
+  float* m_scale;     /* 8 bits only */
+  float* v_scale;
+  void* copy;         /* or null */
+  int64_t n;
+  int16_t param_type, grad_type, copy_type, flags;
+} cnnue_adamw_tensor;
+/* One step over n_tensors tensors (a host array, read during the call; the
+ * launches carry it, so a captured graph holds it).  Every gradient is
+ * multiplied by grad_scale first; when any of d_skip[0..n_skip) is nonzero
+ * nothing changes.  The first form takes the hyper-parameters and the step
+ * (from 1) from the host; the second keeps them in device memory and advances
+ * the step there, as cnnue_adamw_device_scaled does (skipped steps do not
+ * count).  No device memory is allocated, nothing synchronises. */
+int cnnue_adamw_multi(const cnnue_adamw_tensor* tensors, int64_t n_tensors, int state_bits, double lr, double beta1,
+                      double beta2, double eps, double weight_decay, int64_t step, float grad_scale,
+                      const float* d_skip, int n_skip, void* stream);
+int cnnue_adamw_multi_device(const cnnue_adamw_tensor* tensors, int64_t n_tensors, int state_bits,
+                             cnnue_adamw_state* d_state, float grad_scale, const float* d_skip, int n_skip,
+                             void* stream);
 
 /* ---- reference-native AZ-NNUE evaluator (src/az.rs, src/nnue.rs) -------- */
 /* Squares are rank * 9 + file with rank 0 the first rank of a FEN (Black's

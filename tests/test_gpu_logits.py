@@ -1,0 +1,535 @@
+"""process_logits, policy_loss and policy_loss_grad against plain 64-bit forms
+(tests/_logitsref.py), at the sizes, types, strides and masks where rows,
+slices and vectors end."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests import _logitsref as ref
+from chineseai_b200 import logits as lg
+from chineseai_b200._lib import CnnueError
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+SIZES = [(1, 1), (3, 2), (5, 7), (2, 8), (4, 31), (3, 33), (7, 2086), (2, 8100), (3, 8192), (2, 8193), (2, 50001)]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def dev(x):
+    return None if x is None else x.to(DEV)
+
+
+def rows(r, v, dtype, g, pad=0, offset=0):
+    """[r, v] logits inside a larger buffer: row stride v + pad, `offset` elements in."""
+    buf = torch.randn(offset + r * (v + pad) + 16, generator=g) * 3
+    return buf.to(dtype)[offset:offset + r * (v + pad)].view(r, v + pad)[:, :v]
+
+
+def to_dev_strided(x, pad, offset):
+    """x on the device with the same padding and offset."""
+    r, v = x.shape
+    buf = torch.full((offset + r * (v + pad) + 16,), 77.0, dtype=x.dtype, device=DEV)
+    y = buf[offset:offset + r * (v + pad)].view(r, v + pad)[:, :v]
+    y.copy_(x)
+    return y, buf
+
+
+def history_of(r, v, n, g, dtype=torch.int32):
+    h = (torch.rand(r, n, generator=g) ** 3 * v).long().clamp(0, v - 1)
+    h[torch.rand(r, n, generator=g) < 0.05] = -1
+    return h.to(dtype)
+
+
+def mask_of(r, v, share, g):
+    return lg.pack_mask(torch.rand(r, v, generator=g) < share)
+
+
+# ---- process_logits -------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", SIZES)
+def test_process_sizes(size, dtype):
+    R, V = size
+    g = gen(V * 7 + R)
+    x = rows(R, V, dtype, g)
+    kw = dict(history=history_of(R, V, 37, g), lengths=torch.randint(0, 38, (R,), generator=g).int(),
+              prompt_lengths=torch.randint(0, 30, (R,), generator=g).int(), repetition=1 + torch.rand(R, generator=g),
+              frequency=torch.rand(R, generator=g), presence=torch.rand(R, generator=g) - 0.5,
+              bias_tokens=torch.randint(-1, V, (R, 9), generator=g).int(), bias_values=torch.randn(R, 9, generator=g),
+              mask=mask_of(R, V, 0.6, g))
+    out = lg.process_logits(dev(x), **{k: dev(t) for k, t in kw.items()})
+    assert out.dtype == dtype
+    want, bound = ref.process(x, **kw)
+    ref.close(out, want, bound, dtype)
+
+
+@pytest.mark.parametrize("part", ["none", "history", "bias", "mask", "history+mask", "bias+mask", "history+bias"])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_process_parts(part, dtype):
+    R, V = 5, 2086
+    g = gen(len(part))
+    x = rows(R, V, dtype, g)
+    kw = {}
+    if "history" in part:
+        kw.update(history=history_of(R, V, 300, g, torch.int64), repetition=0.5 + torch.rand(R, generator=g))
+    if "bias" in part:
+        kw.update(bias_tokens=torch.randperm(V, generator=g)[:40].int(), bias_values=torch.randn(40, generator=g))
+    if "mask" in part:
+        kw.update(mask=mask_of(1, V, 0.02, g)[0])
+    out = lg.process_logits(dev(x), out_dtype=torch.float32, **{k: dev(t) for k, t in kw.items()})
+    want, bound = ref.process(x, **kw)
+    ref.close(out, want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pad,offset", [(0, 1), (3, 0), (5, 3), (8, 8)])
+def test_process_strides_in_place_and_neighbours(pad, offset, dtype):
+    R, V = 6, 1003
+    g = gen(pad * 10 + offset)
+    x = rows(R, V, dtype, g)
+    kw = dict(history=history_of(R, V, 50, g), frequency=torch.rand(R, generator=g), mask=mask_of(3, V, 0.5, g),
+              mask_index=torch.tensor([2, -1, 0, 1, -5, 2], dtype=torch.int32))
+    want, bound = ref.process(x, **kw)
+    d = {k: dev(t) for k, t in kw.items()}
+    y, buf = to_dev_strided(x, pad, offset)
+    before = buf.clone()
+    ref.close(lg.process_logits(y, **d), want, bound, dtype)
+    assert torch.equal(buf, before), "the logits were written"
+    o, obuf = to_dev_strided(torch.zeros(R, V, dtype=dtype), pad + 1, 2)
+    marks = obuf.clone()
+    lg.process_logits(y, out=o, **d)
+    ref.close(o, want, bound, dtype)
+    o.copy_(marks[2:2 + R * (V + pad + 1)].view(R, -1)[:, :V])
+    assert torch.equal(obuf, marks), "wrote outside the rows"
+    assert lg.process_logits(y, out=y, **d) is y
+    ref.close(y, want, bound, dtype)
+    y.copy_(x)
+    assert torch.equal(buf, before), "in place: wrote outside the rows"
+
+
+def test_process_broadcast_row_and_transposed_logits():
+    g = gen(5)
+    x = rows(1, 500, torch.float32, g)
+    m = mask_of(4, 500, 0.5, g)
+    want, bound = ref.process(x.expand(4, -1), mask=m)
+    ref.close(lg.process_logits(dev(x).expand(4, -1), mask=dev(m)), want, bound)
+    t = torch.randn(500, 4, generator=g)
+    want, bound = ref.process(t.t(), mask=m)
+    ref.close(lg.process_logits(dev(t).t(), mask=dev(m)), want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_process_extremes(dtype):
+    """Infinities, NaN, the type's lowest value, in allowed and masked places; a row that allows nothing."""
+    V = 70
+    lowest = torch.finfo(dtype).min
+    x = torch.zeros(4, V, dtype=dtype)
+    x[:, :6] = torch.tensor([math.inf, -math.inf, math.nan, lowest, -0.0, 1.0]).to(dtype)
+    a = torch.ones(4, V, dtype=torch.bool)
+    a[1] = False
+    a[2, :4] = False
+    a[3] = False
+    a[3, 69] = True
+    h = torch.tensor([0, 1, 2, 3, 4, 5], dtype=torch.int32)
+    kw = dict(history=h, repetition=torch.full((4,), 2.0), mask=lg.pack_mask(a))
+    out = lg.process_logits(dev(x), **{k: dev(t) for k, t in kw.items()}).cpu()
+    assert (out[1] == -math.inf).all()
+    assert (out[2, :4] == -math.inf).all() and (out[2, 6:] == 0).all()
+    assert (out[3, :69] == -math.inf).all() and out[3, 69] == 0
+    assert out[0, 0] == math.inf and out[0, 1] == -math.inf and math.isnan(out[0, 2]) and out[0, 5] == 0.5
+    assert out[0, 3] == -math.inf or dtype == torch.float32 and out[0, 3] == torch.tensor(lowest) * 2
+
+
+def test_process_repeated_bias_tokens_in_list_order():
+    """1e8 + 1 - 1e8: the order of fp32 additions shows."""
+    x = torch.zeros(1, 40)
+    tok = torch.tensor([[3, 3, 5, 3, -1, 5, 39]], dtype=torch.int32)
+    val = torch.tensor([[1e8, 1.0, 2.0, -1e8, 9.0, 0.5, 7.0]])
+    out = lg.process_logits(dev(x), bias_tokens=dev(tok), bias_values=dev(val)).cpu()
+    want = torch.zeros(1, 40)
+    want[0, 3] = (torch.tensor(1e8) + 1.0) - 1e8
+    want[0, 5], want[0, 39] = 2.5, 7.0
+    assert torch.equal(out, want)
+
+
+def test_process_one_token_many_times():
+    V, L = 4096, 100_000
+    x = torch.full((2, V), 1.0)
+    h = torch.full((2, L), 17, dtype=torch.int64)
+    kw = dict(history=dev(h), lengths=dev(torch.tensor([L, 1], dtype=torch.int32)),
+              prompt_lengths=dev(torch.tensor([5, 1], dtype=torch.int32)), frequency=dev(torch.full((2,), 0.5)),
+              presence=dev(torch.full((2,), 0.25)), repetition=dev(torch.full((2,), 2.0)))
+    out = lg.process_logits(dev(x), **kw).cpu()
+    assert out[0, 17] == 0.5 - 0.5 * (L - 5) - 0.25 and out[1, 17] == 0.5
+    out[:, 17] = 1.0
+    assert (out == 1.0).all()
+
+
+def test_process_bad_data_is_reported_and_skipped():
+    x = torch.ones(3, 50)
+    h = torch.tensor([[1, 50, 2], [3, 2**31 - 1, 4], [5, 6, 7]], dtype=torch.int32)
+    f = torch.ones(3)
+    with pytest.raises(CnnueError, match="index"):
+        lg.process_logits(dev(x), history=dev(h), frequency=dev(f))
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    wide = h.long()
+    wide[1, 1] = 2**40
+    out = lg.process_logits(dev(x), history=dev(wide), frequency=dev(f), status=status).cpu()
+    want = torch.ones(3, 50)
+    for r, ts in enumerate(([1, 2], [3, 4], [5, 6, 7])):
+        want[r, ts] = 0.0
+    assert torch.equal(out, want) and int(status) == 1
+    status.zero_()
+    out = lg.process_logits(dev(x), history=dev(h[2:3].expand(3, 3).contiguous()), frequency=dev(f), status=status,
+                            lengths=dev(torch.tensor([-1, 4, 1], dtype=torch.int32))).cpu()
+    assert int(status) == 2
+    assert (out[0] == 1).all() and (out[1, 5:8] == 0).all() and out[2, 5] == 0 and (out[2, 6:8] == 1).all()
+    status.zero_()
+    out = lg.process_logits(dev(x), bias_tokens=dev(torch.tensor([50, 4], dtype=torch.int32)),
+                            bias_values=dev(torch.tensor([3.0, 1.0])), status=status).cpu()
+    assert int(status) == 1 and out[0, 4] == 2 and out.sum() == 153
+    status.zero_()
+    m = lg.pack_mask(torch.ones(2, 50, dtype=torch.bool))
+    out = lg.process_logits(dev(x), mask=dev(m), mask_index=dev(torch.tensor([0, 2, 1], dtype=torch.int32)),
+                            status=status).cpu()
+    assert int(status) == 1 and (out[1] == -math.inf).all() and (out[[0, 2]] == 1).all()
+
+
+def test_process_empty():
+    assert lg.process_logits(torch.empty(0, 5, device=DEV)).shape == (0, 5)
+    x = torch.ones(2, 9, device=DEV)
+    none = torch.empty(2, 0, dtype=torch.int32, device=DEV)
+    out = lg.process_logits(x, history=none, frequency=torch.ones(2, device=DEV), bias_tokens=none,
+                            bias_values=torch.empty(2, 0, device=DEV))
+    assert torch.equal(out, x)
+
+
+def test_process_long_history_and_large_vocabulary():
+    R, V, L = 3, 200_003, 20_000
+    g = gen(9)
+    x = rows(R, V, torch.bfloat16, g)
+    kw = dict(history=history_of(R, V, L, g), frequency=torch.rand(R, generator=g), repetition=1 + torch.rand(R, generator=g),
+              prompt_lengths=torch.tensor([0, 10_000, 20_000], dtype=torch.int32),
+              bias_tokens=torch.randint(0, V, (R, 300), generator=g).int(), bias_values=torch.randn(R, 300, generator=g),
+              mask=mask_of(R, V, 0.9, g))
+    want, bound = ref.process(x, **kw)
+    ref.close(lg.process_logits(dev(x), **{k: dev(t) for k, t in kw.items()}), want, bound, torch.bfloat16)
+
+
+def test_process_captured_and_replayed_on_new_data():
+    g = gen(3)
+    R, V = 4, 2086
+    x, h, n = dev(rows(R, V, torch.float32, g)), dev(history_of(R, V, 64, g)), dev(torch.full((R,), 10, dtype=torch.int32))
+    f = dev(torch.rand(R, generator=g))
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = torch.empty_like(x)
+    lg.process_logits(x, history=h, lengths=n, frequency=f, out=out, status=status)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lg.process_logits(x, history=h, lengths=n, frequency=f, out=out, status=status)
+    for k in (20, 64):
+        n.fill_(k)
+        x.mul_(0.5)
+        graph.replay()
+        want, bound = ref.process(x.cpu(), history=h.cpu(), lengths=n.cpu(), frequency=f.cpu())
+        ref.close(out, want, bound)
+    assert int(status) == 0
+
+
+def test_process_on_another_stream():
+    g = gen(4)
+    x = rows(64, 8100, torch.float32, g)
+    m = mask_of(64, 8100, 0.3, g)
+    want, bound = ref.process(x, mask=m)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        out = lg.process_logits(x.to(DEV), mask=m.to(DEV), status=torch.zeros(1, dtype=torch.int32, device=DEV))
+    s.synchronize()
+    ref.close(out, want, bound)
+
+
+# ---- policy_loss ------------------------------------------------------------------
+def loss_inputs(R, V, dtype, kind, g, pad=0, share=0.5):
+    x = rows(R, V, dtype, g, pad)
+    kw = {}
+    if kind == "dense":
+        kw["targets"] = torch.rand(R, V, generator=g) ** 2
+    elif kind == "dense16":
+        kw["targets"] = (torch.rand(R, V, generator=g) ** 2).to(torch.bfloat16 if dtype != torch.float16 else dtype)
+    elif kind == "labels":
+        kw["target_index"] = torch.randint(-1 if R > 1 else 0, V, (R,), generator=g)
+    else:
+        kw["target_index"] = torch.randint(-1, V, (R, 17), generator=g).int()
+        kw["target_prob"] = torch.rand(R, 17, generator=g)
+    if share < 1:
+        kw["mask"] = mask_of(R, V, share, g)
+    kw["weights"] = torch.rand(R, generator=g) + 0.25
+    return x, kw
+
+
+def check_all(x, kw, dtype, up=None):
+    """The fused form and autograd against the 64-bit form."""
+    R = x.shape[0]
+    d = {k: dev(t) for k, t in kw.items()}
+    want, grad, b_loss, b_grad = ref.loss(x, **kw)
+    loss, got = lg.policy_loss_grad(dev(x), d.pop("targets", None), **d)
+    ref.close(loss, want, b_loss)
+    ref.close(got, grad, b_grad, dtype)
+    up = torch.linspace(-1, 2, R) if up is None else up
+    _, grad, _, b_grad = ref.loss(x, **kw, upstream=up)
+    leaf = dev(x).requires_grad_(True)
+    d = {k: dev(t) for k, t in kw.items()}
+    loss = lg.policy_loss(leaf, d.pop("targets", None), **d)
+    ref.close(loss, want, b_loss)
+    (got,) = torch.autograd.grad(loss, leaf, dev(up))
+    ref.close(got, grad, b_grad, dtype)
+
+
+@pytest.mark.parametrize("kind", ["dense", "dense16", "labels", "lists"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", SIZES)
+def test_loss_sizes(size, dtype, kind):
+    g = gen(size[1] + size[0] * 3)
+    x, kw = loss_inputs(*size, dtype, kind, g)
+    check_all(x, kw, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_loss_large_vocabulary(dtype):
+    g = gen(11)
+    x, kw = loss_inputs(2, 140_001, dtype, "lists", g, share=1.0)
+    check_all(x, kw, dtype)
+    x, kw = loss_inputs(1, 300_007, dtype, "dense", g, share=0.9)
+    check_all(x, kw, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pad,offset", [(0, 1), (3, 0), (5, 3)])
+def test_loss_strides_and_neighbours(pad, offset, dtype):
+    R, V = 5, 2087
+    g = gen(pad + offset)
+    x, kw = loss_inputs(R, V, dtype, "dense", g)
+    want, grad, b_loss, b_grad = ref.loss(x, **kw)
+    d = {k: dev(t) for k, t in kw.items()}
+    y, _ = to_dev_strided(x, pad, offset)
+    t, _ = to_dev_strided(kw["targets"], 1, 3)
+    d.pop("targets")
+    o, obuf = to_dev_strided(torch.zeros(R, V, dtype=dtype), pad, 2)
+    marks = obuf.clone()
+    loss, got = lg.policy_loss_grad(y, t, grad=o, **d)
+    assert got is o
+    ref.close(loss, want, b_loss)
+    ref.close(o, grad, b_grad, dtype)
+    o.copy_(marks[2:2 + R * (V + pad)].view(R, -1)[:, :V])
+    assert torch.equal(obuf, marks), "wrote outside the gradient"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_loss_of_a_common_offset_keeps_its_digits(dtype):
+    g = gen(2)
+    x = (torch.randn(3, 2086, generator=g) + 1000).to(dtype)
+    check_all(x, {"target_index": torch.tensor([5, 0, 2085]), "mask": mask_of(3, 2086, 0.9, g) | -1}, dtype)
+
+
+@pytest.mark.parametrize("kind", ["dense", "labels", "lists"])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_loss_rows_where_little_or_nothing_is_left(kind, dtype):
+    """Nothing allowed; only -inf allowed; NaN and infinities in masked places; weight 0 over NaN; the lowest value;
+    one token; no target; targets all masked."""
+    R, V = 10, 1000
+    g = gen(6)
+    x, kw = loss_inputs(R, V, dtype, kind, g, share=2.0)
+    lowest = torch.finfo(dtype).min
+    a = torch.rand(R, V, generator=g) < 0.5
+    a[:, 7] = True
+    a[0] = False
+    x[1] = -math.inf
+    x[2][~a[2]] = math.nan
+    x[3][~a[3]] = math.inf
+    x[4] = math.nan
+    kw["weights"][4] = 0.0
+    x[5] = lowest
+    a[6] = False
+    a[6, 7] = True
+    if kind == "dense":
+        kw["targets"][7] = 0.0
+        kw["targets"][8] = torch.where(a[8], 0.0, kw["targets"][8])
+        kw["targets"][2][~a[2]] = math.nan
+    else:
+        kw["target_index"][7] = -1
+        kw["target_index"][8] = int((~a[8]).nonzero()[0])
+    kw["mask"] = lg.pack_mask(a)
+    if kind == "dense":  # the plain form multiplies: give it zeros where the operator must not look
+        clean = dict(kw, targets=torch.where(a, kw["targets"], 0.0))
+    else:
+        clean = kw
+    want, grad, b_loss, b_grad = ref.loss(torch.where(a, x, torch.zeros((), dtype=dtype)), **clean)
+    d = {k: dev(t) for k, t in kw.items()}
+    loss, got = lg.policy_loss_grad(dev(x), d.pop("targets", None), **d)
+    ref.close(loss, want, b_loss)
+    ref.close(got, grad, b_grad, dtype)
+    for r in (0, 1, 4, 7, 8):
+        assert float(loss[r]) == 0 and not got[r].any()
+    leaf = dev(x).requires_grad_(True)
+    d = {k: dev(t) for k, t in kw.items()}
+    loss = lg.policy_loss(leaf, d.pop("targets", None), **d)
+    ref.close(loss, want, b_loss)
+    loss.sum().backward()
+    ref.close(leaf.grad, grad, b_grad, dtype)
+
+
+def test_loss_nan_and_infinite_logits_at_allowed_tokens():
+    x = torch.zeros(4, 64)
+    x[0, 3] = math.nan
+    x[1, 3] = math.inf
+    x[2, 3] = -math.inf  # no target there
+    x[3, 5] = -math.inf  # a target there
+    label = torch.tensor([5, 5, 5, 5])
+    loss, grad = lg.policy_loss_grad(dev(x), target_index=dev(label))
+    loss, grad = loss.cpu(), grad.cpu()
+    assert math.isnan(loss[0]) and grad[0].isnan().all()
+    assert math.isnan(loss[1]) or loss[1] == math.inf
+    assert abs(float(loss[2]) - math.log(63)) < 1e-6 and grad[2, 3] == 0
+    assert loss[3] == math.inf and grad[3, 5] == -1 and abs(float(grad[3, 0]) - 1 / 63) < 1e-7
+
+
+def test_loss_masses_other_than_one_and_repeated_tokens():
+    g = gen(8)
+    x = torch.randn(3, 100, generator=g)
+    kw = dict(target_index=torch.tensor([[4, 4, 4, 9], [0, 99, 0, 99], [-1, 3, -1, 3]]),
+              target_prob=torch.tensor([[0.5, 2.0, -1.0, 0.1], [3.0, 0.0, 1.0, 0.25], [5.0, 0.5, 5.0, 0.5]]))
+    check_all(x, kw, torch.float32)
+
+
+def test_loss_gradient_against_differences():
+    g = gen(10)
+    x = torch.randn(2, 40, generator=g)
+    kw = dict(target_index=torch.randint(0, 40, (2, 5), generator=g), target_prob=torch.rand(2, 5, generator=g),
+              mask=mask_of(2, 40, 0.7, g), weights=torch.tensor([0.7, 1.3]))
+    _, grad = lg.policy_loss_grad(dev(x), **{k: dev(t) for k, t in kw.items()})
+    h = 1e-5
+    for j in range(40):
+        up, down = x.double().clone(), x.double().clone()
+        up[:, j] += h
+        down[:, j] -= h
+        d = (ref.loss(up, **kw)[0] - ref.loss(down, **kw)[0]) / (2 * h)
+        # third derivative of the loss is at most 1 (times weight and mass): h^2; the kernel's own bound above it
+        ref.close(grad[:, j], d, torch.full((2,), 8 * h * h + 1e-10 / h + 1e-6).double())
+
+
+def test_loss_broadcast_logits_sum_their_gradients():
+    g = gen(12)
+    x = torch.randn(1, 333, generator=g)
+    label = torch.randint(0, 333, (6,), generator=g)
+    leaf = dev(x).requires_grad_(True)
+    lg.policy_loss(leaf.expand(6, -1), target_index=dev(label)).sum().backward()
+    _, grad, _, b = ref.loss(x.expand(6, -1), target_index=label)
+    ref.close(leaf.grad, grad.sum(0, keepdim=True), b.sum(0, keepdim=True) + 6 * ref.EPS32 * grad.abs().sum(0, keepdim=True))
+
+
+def test_loss_bad_tokens_are_reported_and_skipped():
+    x = torch.zeros(2, 50)
+    t = torch.tensor([[3, 50], [2**40, 4]])
+    with pytest.raises(CnnueError, match="index"):
+        lg.policy_loss(dev(x), target_index=dev(t))
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    loss, grad = lg.policy_loss_grad(dev(x), target_index=dev(t), status=status)
+    assert int(status) == 1
+    want, g, bl, bg = ref.loss(x, target_index=torch.tensor([[3, -1], [-1, 4]]))
+    ref.close(loss, want, bl)
+    ref.close(grad, g, bg)
+
+
+def test_loss_empty():
+    loss, grad = lg.policy_loss_grad(torch.empty(0, 5, device=DEV), target_index=torch.empty(0, dtype=torch.int64, device=DEV))
+    assert loss.shape == (0,) and grad.shape == (0, 5)
+    x = torch.randn(2, 9, device=DEV)
+    loss, grad = lg.policy_loss_grad(x, target_index=torch.empty(2, 0, dtype=torch.int32, device=DEV))
+    assert not loss.any() and not grad.any()
+
+
+def test_loss_step_captured_and_replayed():
+    g = gen(13)
+    x, kw = loss_inputs(8, 2086, torch.bfloat16, "lists", g)
+    d = {k: dev(t) for k, t in kw.items()}
+    y = dev(x).clone()
+    grad = torch.empty_like(y)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    lg.policy_loss_grad(y, grad=grad, status=status, **d)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, _ = lg.policy_loss_grad(y, grad=grad, status=status, **d)
+    y.mul_(0.5)
+    graph.replay()
+    want, gr, bl, bg = ref.loss(y.cpu(), **kw)
+    ref.close(loss, want, bl)
+    ref.close(grad, gr, bg, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_results_do_not_change_from_run_to_run(dtype):
+    g = gen(14)
+    x, kw = loss_inputs(33, 30_011, dtype, "lists", g)
+    d = {k: dev(t) for k, t in kw.items()}
+    first = lg.policy_loss_grad(dev(x), **d)
+    for _ in range(3):
+        again = lg.policy_loss_grad(dev(x), **d)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+# ---- together, as they are used -----------------------------------------------------
+def test_legal_moves_choose_learn_and_update():
+    """The ResNet's logits under the rules of the game: legal-move priors; then
+    a policy head learns visit counts under the same masks, with 8-bit AdamW."""
+    from chineseai_b200 import az, mcts, resnet
+    from chineseai_b200.optim import MultiAdamW
+    n = 6
+    boards = az.random_boards(n, 3)
+    sides = np.arange(n, dtype=np.uint8) % 2
+    mask = torch.from_numpy(mcts.legal_mask(boards, sides)).to(DEV)
+    model = resnet.ResNetModel(resnet.ResNetWeights.synthetic(5))
+    planes = torch.from_numpy(resnet.synthetic_planes(n, 6).view(np.int16)).to(DEV)
+    probs, logits, _ = model.forward(planes, with_logits=True)
+    a = ref.unpack(mask.cpu(), 2086)
+    want, bound = ref.process(logits.cpu(), mask=mask.cpu())
+    ref.close(lg.process_logits(logits, mask=mask), want, bound)
+    model.close()
+
+    g = gen(1)
+    feats = torch.randn(n, 32, generator=g)
+    head = [torch.randn(2086, 32, generator=g) * 0.1, torch.zeros(2086)]
+    visits = torch.rand(n, 2086, generator=g) * a
+    visits = visits / visits.sum(1, keepdim=True).clamp(min=1e-9)
+    w = torch.full((n,), 1.0 / n)
+    p = [dev(t).clone() for t in head]
+    grads = [torch.empty_like(t) for t in p]
+    opt = MultiAdamW(p, grads, lr=1e-2, state_bits=8)
+    z = torch.addmm(p[1], dev(feats), p[0].t())
+    loss, gz = lg.policy_loss_grad(z, dev(visits), mask=mask, weights=dev(w))
+    torch.mm(gz.t(), dev(feats), out=grads[0])
+    torch.sum(gz, 0, out=grads[1])
+    opt.step()
+    # the same step in 64 bits
+    hp = [t.double().requires_grad_(True) for t in head]
+    zz = torch.addmm(hp[1], feats.double(), hp[0].t()).masked_fill(~a, -math.inf)
+    lse = torch.logsumexp(zz, 1, keepdim=True)
+    total = (-(visits.double() * torch.where(a, zz - lse, 0.0)).sum(1) * w.double())
+    total.sum().backward()
+    # logits differ by the fp32 matmul's rounding (33 terms of size < 5) and so does the loss
+    assert (loss.cpu().double() - total.detach()).abs().max() < 40 * 5 * 33 * ref.EPS32
+    for q, h, gr in zip(p, hp, grads):
+        # gradients: the fp32 sum over the boards and the logits' error
+        assert (gr.cpu().double() - h.grad).abs().max() < 1e-4 * h.grad.abs().max()
+        # a first AdamW step moves every parameter by lr * g / (|g| + eps), less the decay
+        g64 = gr.cpu().double()
+        step = h.detach() * (1 - 1e-2 * 1e-4) - 1e-2 * g64 / (g64.abs() + 1e-8)
+        # below 2^-60 the squares leave fp32's normal range and the root loses digits
+        big = (g64.abs() > 2.0 ** -55) | (g64 == 0)
+        assert ((q.cpu().double() - step).abs()[big] <= 16 * ref.EPS32 * (step.abs() + 1e-2)[big]).all()
