@@ -2,6 +2,8 @@
 // biases and masks on rows of logits, and the masked softmax cross entropy
 // with its gradient.  Rows are [vocab] of fp32, bf16 or fp16 at any stride;
 // arithmetic is fp32, rounded once at the store.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "rowvec.cuh"
@@ -10,6 +12,7 @@ namespace cnnue {
 namespace logits {
 namespace {
 
+namespace cg = cooperative_groups;
 using rows::kNegInf;
 using rows::Vec;
 
@@ -209,12 +212,11 @@ int pick_process(ProcArgs& a, int64_t n_rows, cudaStream_t s) {
 // does not cancel.
 // ---------------------------------------------------------------------------
 
-constexpr int kLossThreads = 256;
-
 struct LossArgs {
   const void* z;
   int64_t z_stride;
   int vocab;
+  int split, vps;         // slices (CTAs) per row, vectors per slice
   cnnue_loss_targets t;
   const float* upstream;  // [rows] or null (backward pass)
   float* loss;            // [rows] or null
@@ -223,16 +225,6 @@ struct LossArgs {
   int64_t grad_stride;
   uint32_t* status;
 };
-
-template <typename T>
-__device__ __forceinline__ float target_at(const void* p, int64_t i) {
-  return Vec<T>::up(((const T*)p)[i]);
-}
-__device__ __forceinline__ float dense_target(const cnnue_loss_targets& t, int64_t i) {
-  return t.dense_type == CNNUE_F32    ? target_at<float>(t.dense, i)
-         : t.dense_type == CNNUE_BF16 ? target_at<__nv_bfloat16>(t.dense, i)
-                                      : target_at<__half>(t.dense, i);
-}
 
 struct RowMask {
   const uint32_t* words;  // null: everything is allowed (unless dead)
@@ -255,167 +247,421 @@ __device__ __forceinline__ bool token_ok(const RowMask& m, int t) {
 }
 
 struct Sums {
-  float m, s, t, d;  // running maximum, sum of exp(z - m), target mass, sum of t (m - z)
+  float m, s, t, d;  // maximum, sum of exp(z - m), target mass, sum of t (m - z)
 };
-// a += b, both relative to their own maxima.
-__device__ __forceinline__ void join(Sums& a, const Sums& b) {
-  const float m = rows::max_nan(a.m, b.m);
-  if (m == kNegInf) {
-    a.t += b.t;
-    return;
-  }
-  const float fa = a.m == m ? 1.f : exp2f((a.m - m) * rows::kLog2e), fb = b.m == m ? 1.f : exp2f((b.m - m) * rows::kLog2e);
-  // a side without allowed logits above -inf has s = 0; its mass sits on -inf logits
-  a.d = (a.t != 0.f ? a.d + a.t * (m - a.m) : 0.f) + (b.t != 0.f ? b.d + b.t * (m - b.m) : 0.f);
-  a.s = a.s * fa + b.s * fb;
-  a.t += b.t;
-  a.m = m;
-}
 
-__device__ __forceinline__ Sums block_join(Sums v, Sums* shared) {
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float lane_sum(float x) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    Sums u;
-    u.m = __shfl_xor_sync(~0u, v.m, o);
-    u.s = __shfl_xor_sync(~0u, v.s, o);
-    u.t = __shfl_xor_sync(~0u, v.t, o);
-    u.d = __shfl_xor_sync(~0u, v.d, o);
-    // both lanes of a pair form the same sum in the same order
-    if (threadIdx.x & o) {
-      join(u, v);
-      v = u;
-    } else {
-      join(v, u);
-    }
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+  return x;
+}
+// The sums of 32 lanes, each relative to its own maximum, as one; every lane
+// gets the same bits.  A side without a logit above -inf has s = 0; mass that
+// sits on its -inf logits makes d infinite, as t (m - z) says.
+__device__ __forceinline__ Sums join_lanes(Sums v) {
+  float m;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v.m));
+  if (m != kNegInf) {
+    v.s = v.m == kNegInf ? 0.f : v.s * exp2_fast((v.m - m) * rows::kLog2e);
+    v.d = v.t != 0.f ? v.d + v.t * (m - v.m) : 0.f;
   }
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = shared[0];
-  for (int w = 1; w < kLossThreads / 32; ++w) join(v, shared[w]);
+  v.m = m;
+  v.s = lane_sum(v.s);
+  v.t = lane_sum(v.t);
+  v.d = lane_sum(v.d);
   return v;
 }
+__device__ __forceinline__ Sums nothing() { return {kNegInf, 0.f, 0.f, 0.f}; }
 
-// One CTA per row.  FWD: the row's sums, loss and stats.  GRAD: the gradient
-// (with !FWD from the stats of an earlier forward pass).
-template <typename T, bool FWD, bool GRAD>
-__global__ void __launch_bounds__(kLossThreads) loss_kernel(const LossArgs a) {
-  constexpr int VE = Vec<T>::VE;
-  __shared__ Sums shared[kLossThreads / 32];
-  const int64_t row = blockIdx.x;
-  const T* z = (const T*)a.z + row * a.z_stride;
-  const int shift = rows::shift_of(z);
-  const int nv = (shift + a.vocab + VE - 1) / VE;
-  const bool wide = a.t.index_bytes == 8;
-  const char* list = a.t.index ? (const char*)a.t.index + row * a.t.index_stride * a.t.index_bytes : nullptr;
-  const float* prob = a.t.prob ? a.t.prob + row * a.t.prob_stride : nullptr;
-  float w = a.t.weights ? a.t.weights[row] : 1.f;
-  const bool idle = w == 0.f;  // a padded row: not read, loss and gradient 0
-  const RowMask mask = row_mask(a.t, row, a.status, threadIdx.x == 0);
+// The sums of the CTA's threads; then of the CTAs of its cluster, whose
+// `shared[32]` every CTA reads over distributed shared memory.  The caller
+// waits for the cluster (cluster_done) before it leaves.
+__device__ __forceinline__ Sums join_all(Sums v, Sums* shared, int ctas) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  v = join_lanes(v);
+  if (lane == 0) shared[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = join_lanes(lane < warps ? shared[lane] : nothing());
+  if (ctas > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    if (threadIdx.x == 0) shared[32] = v;
+    cluster.sync();
+    v = join_lanes(lane < ctas ? *cluster.map_shared_rank(shared + 32, lane) : nothing());
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  }
+  return v;
+}
+__device__ __forceinline__ void cluster_done(int ctas) {
+  if (ctas > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
 
-  Sums v{kNegInf, 0.f, 0.f, 0.f};
-  if (FWD && !idle) {
-    for (int i = threadIdx.x; i < nv; i += kLossThreads) {
-      const int e0 = i * VE - shift;
-      const uint32_t in = rows::inside<VE>(e0, a.vocab);
-      const uint32_t ok = mask.dead ? 0 : mask.words ? rows::allowed<VE>(mask.words, e0, a.vocab) : in;
-      if (ok == 0) continue;
-      float x[VE];
-      rows::load(z, e0, in, ok, kNegInf, x);
-      Sums u{x[0], 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 1; j < VE; ++j) u.m = rows::max_nan(u.m, x[j]);
-#pragma unroll
-      for (int j = 0; j < VE; ++j) {
-        if (u.m != kNegInf) u.s += exp2f((x[j] - u.m) * rows::kLog2e);
-        if (a.t.dense && (ok >> j & 1)) {
-          const float t = dense_target(a.t, row * a.t.dense_stride + e0 + j);
-          if (t != 0.f) {
-            u.t += t;
-            if (u.m != kNegInf) u.d += t * (u.m - x[j]);
-          }
-        }
-      }
-      join(v, u);
-    }
-    v = block_join(v, shared);
-    if (list) {  // every thread forms the same sums in list order
-      for (int64_t k = 0; k < a.t.count; ++k) {
-        const int tok = rows::token_at(list, k, wide);
-        if (tok >= a.vocab) {
-          if (threadIdx.x == 0) atomicOr(a.status, CNNUE_STATUS_BAD_INDEX);
-          continue;
-        }
-        const float t = tok < 0 || !token_ok(mask, tok) ? 0.f : prob ? prob[k] : 1.f;
-        if (t != 0.f) {
-          v.t += t;
-          v.d += t * (v.m - Vec<T>::up(z[tok]));
-        }
-      }
-    }
-    if (threadIdx.x == 0) {
-      if (a.loss) a.loss[row] = v.m == kNegInf ? 0.f : w * ((v.t != 0.f ? v.t * logf(v.s) : 0.f) + v.d);
-      if (a.stats) {
-        a.stats[3 * row] = v.m;
-        a.stats[3 * row + 1] = v.s;
-        a.stats[3 * row + 2] = v.t;
-      }
-    }
-  } else if (FWD && threadIdx.x == 0) {
-    if (a.loss) a.loss[row] = 0.f;
-    if (a.stats) a.stats[3 * row] = kNegInf;
+// One row's tensors as a CTA sees them.
+template <typename T>
+struct LossRow {
+  static constexpr int VE = Vec<T>::VE;
+  const LossArgs& a;
+  int64_t row;
+  const T* z;
+  int shift;
+  RowMask mask;
+  const char* list;
+  const float* prob;
+  bool wide;
+
+  __device__ __forceinline__ LossRow(const LossArgs& args, int64_t r, bool tell) : a(args), row(r) {
+    z = (const T*)a.z + row * a.z_stride;
+    shift = rows::shift_of(z);
+    mask = row_mask(a.t, row, a.status, tell);
+    wide = a.t.index_bytes == 8;
+    list = a.t.index ? (const char*)a.t.index + row * a.t.index_stride * a.t.index_bytes : nullptr;
+    prob = a.t.prob ? a.t.prob + row * a.t.prob_stride : nullptr;
   }
-  if (!GRAD) return;
-  if (!FWD) v.m = a.stats[3 * row], v.s = a.stats[3 * row + 1], v.t = a.stats[3 * row + 2];
-  if (a.upstream) w *= a.upstream[row];
-  T* g = (T*)a.grad + row * a.grad_stride;
-  const bool whole = rows::lines_up(g, shift);
-  const bool none = idle || v.m == kNegInf;  // nothing is left of the row
-  const float c = none || v.t == 0.f ? 0.f : w * v.t / v.s;
-  for (int i = threadIdx.x; i < nv; i += kLossThreads) {
-    const int e0 = i * VE - shift;
-    const uint32_t in = rows::inside<VE>(e0, a.vocab);
-    const uint32_t ok = none || mask.dead ? 0 : mask.words ? rows::allowed<VE>(mask.words, e0, a.vocab) : in;
-    float x[VE];
-    rows::load(z, e0, in, c == 0.f ? 0 : ok, kNegInf, x);
-#pragma unroll
-    for (int j = 0; j < VE; ++j) {
-      const float t = a.t.dense && (ok >> j & 1) ? dense_target(a.t, row * a.t.dense_stride + e0 + j) : 0.f;
-      x[j] = ok >> j & 1 ? (c == 0.f ? 0.f : c * exp2f((x[j] - v.m) * rows::kLog2e)) - w * t : 0.f;
-    }
-    rows::store<T, VE>(g, e0, in, whole, x);
+  __device__ __forceinline__ uint32_t allowed(int e0) const {
+    return mask.dead ? 0 : mask.words ? rows::allowed<VE>(mask.words, e0, a.vocab) : rows::inside<VE>(e0, a.vocab);
   }
-  if (!list || none) return;
-  __syncthreads();  // the listed tokens' elements again, now with their targets
-  for (int64_t k = threadIdx.x; k < a.t.count; k += kLossThreads) {
+  // The dense targets of vector e0, 0 where `ok` has no bit.
+  __device__ __forceinline__ void targets(int e0, uint32_t ok, float* t) const {
+    const int64_t at = row * a.t.dense_stride + e0;
+    if (a.t.dense_type == CNNUE_F32)
+      dense_vec<float>(at, ok, t);
+    else if (a.t.dense_type == CNNUE_BF16)
+      dense_vec<__nv_bfloat16>(at, ok, t);
+    else
+      dense_vec<__half>(at, ok, t);
+  }
+  template <typename D>
+  __device__ __forceinline__ void dense_vec(int64_t at, uint32_t ok, float* t) const {
+    constexpr int DE = Vec<D>::VE;
+    const D* p = (const D*)a.t.dense + at;
+    // whole vectors when they line up with the logits' and nothing is masked out of one
+    if (ok == rows::kFull<VE> && VE % DE == 0 && ((uintptr_t)p & 15) == 0) {
+#pragma unroll
+      for (int j = 0; j < VE / DE; ++j) Vec<D>::unpack(__ldg(reinterpret_cast<const uint4*>(p) + j), t + j * DE);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) t[i] = ok >> i & 1 ? Vec<D>::up(p[i]) : 0.f;
+    }
+  }
+  // Entry k of the list: its token, or -1 when it does not count.
+  __device__ __forceinline__ int entry(int64_t k) const {
     const int tok = rows::token_at(list, k, wide);
-    if (tok < 0 || tok >= a.vocab || !token_ok(mask, tok)) continue;
-    float t = 0.f;
-    bool again = false;  // a token named before belongs to its first entry
-    for (int64_t j = 0; j < a.t.count; ++j) {
-      if (rows::token_at(list, j, wide) != tok) continue;
-      if (j < k) {
-        again = true;
-        break;
+    return tok >= 0 && tok < a.vocab && token_ok(mask, tok) ? tok : -1;
+  }
+  __device__ __forceinline__ float mass(int64_t k) const { return prob ? __ldg(prob + k) : 1.f; }
+
+  // Mass and d of the list's entries on tokens [lo, hi), relative to m.
+  __device__ __forceinline__ void list_sums(int lo, int hi, bool tell, Sums& v) const {
+    for (int64_t k = threadIdx.x; k < a.t.count; k += blockDim.x) {
+      if (tell && rows::token_at(list, k, wide) >= a.vocab) atomicOr(a.status, CNNUE_STATUS_BAD_INDEX);
+      const int tok = entry(k);
+      if (tok < lo || tok >= hi) continue;
+      const float t = mass(k);
+      if (t == 0.f) continue;
+      const float x = Vec<T>::up(z[tok]);
+      // relative to this thread's own maximum, which need not be above x
+      if (v.m == kNegInf && x != kNegInf) {
+        v.m = x;  // s = 0
+        v.d = v.t != 0.f ? -kNegInf : 0.f;
       }
-      t += prob ? prob[j] : 1.f;
+      v.t += t;
+      v.d += v.m == kNegInf ? 0.f : t * (v.m - x);
     }
-    if (again) continue;
-    g[tok] = Vec<T>::down((c == 0.f ? 0.f : c * exp2f((Vec<T>::up(z[tok]) - v.m) * rows::kLog2e)) - w * t);
+  }
+
+  // The gradient at the listed tokens [lo, hi): c exp(z - m) - w t, with t
+  // summed in list order by the thread of the token's first entry.
+  __device__ __forceinline__ void list_grads(int lo, int hi, T* g, float m, float c, float w) const {
+    for (int64_t k = threadIdx.x; k < a.t.count; k += blockDim.x) {
+      const int tok = entry(k);
+      if (tok < lo || tok >= hi) continue;
+      float t = 0.f;
+      int64_t j = 0;
+      while (j < k && rows::token_at(list, j, wide) != tok) ++j;
+      if (j < k) continue;  // an earlier entry's
+      for (; j < a.t.count; ++j)
+        if (rows::token_at(list, j, wide) == tok) t += mass(j);
+      g[tok] = Vec<T>::down((c == 0.f ? 0.f : c * exp2_fast((Vec<T>::up(z[tok]) - m) * rows::kLog2e)) - w * t);
+    }
+  }
+};
+
+// exp(x - m) of a vector (m finite or NaN); *sum gets their sum.
+template <int VE>
+__device__ __forceinline__ void exps(float* x, float m, float2* sum) {
+  const float2 minus = make_float2(-m, -m), scale = make_float2(rows::kLog2e, rows::kLog2e);
+#pragma unroll
+  for (int j = 0; j < VE; j += 2) {
+    float2 d = rows::mul2(rows::add2(make_float2(x[j], x[j + 1]), minus), scale);
+    d.x = exp2_fast(d.x);
+    d.y = exp2_fast(d.y);
+    if (sum) *sum = rows::add2(*sum, d);
+    x[j] = d.x;
+    x[j + 1] = d.y;
+  }
+}
+template <int VE>
+__device__ __forceinline__ float top_of(const float* x, float m) {
+#pragma unroll
+  for (int j = 0; j < VE; j += 2) m = rows::max_nan(m, x[j], x[j + 1]);
+  return m;
+}
+
+// The gradient's vector e0 from the raw logits: c exp(z - m) - w t on `ok`, 0
+// elsewhere.  c = 0: nothing but the targets (and the logits are not looked
+// at, so no NaN comes from them).
+template <typename T, bool DENSE>
+__device__ __forceinline__ void grad_vector(const LossRow<T>& r, const uint4& raw, int e0, uint32_t ok, float m, float c,
+                                            float w, float* x) {
+  constexpr int VE = Vec<T>::VE;
+  if (c != 0.f && ok) {
+    Vec<T>::unpack(raw, x);
+    exps<VE>(x, m, nullptr);
+#pragma unroll
+    for (int j = 0; j < VE; j += 2) {
+      const float2 e = rows::mul2(make_float2(x[j], x[j + 1]), make_float2(c, c));
+      x[j] = e.x;
+      x[j + 1] = e.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VE; ++j) x[j] = 0.f;
+  }
+  if (DENSE && ok) {
+    float t[VE];
+    r.targets(e0, ok, t);
+#pragma unroll
+    for (int j = 0; j < VE; ++j) x[j] -= w * t[j];
+  }
+  if (ok != rows::kFull<VE>) {
+#pragma unroll
+    for (int j = 0; j < VE; ++j)
+      if (!(ok >> j & 1)) x[j] = 0.f;
   }
 }
 
-template <typename T, bool FWD, bool GRAD>
-int launch_loss(const LossArgs& a, int64_t n_rows, cudaStream_t s) {
-  if (n_rows > 0x7fffffff) return set_error(CNNUE_ERR_INVALID_ARG, "too many rows for one call");
-  loss_kernel<T, FWD, GRAD><<<(unsigned)n_rows, kLossThreads, 0, s>>>(a);
+constexpr int kLossThreads = 256;
+
+// Loss, and with GRAD the gradient, of one slice of a row; the slices of a row
+// are the CTAs of a cluster.  A thread takes every blockDim-th vector of the
+// slice.  KEEP: it copies them into shared memory, all in flight at once, and
+// reads them there twice: for the row's sums (online, relative to the thread's
+// running maximum) and, once the cluster has joined those, for the gradient;
+// the row is read from memory once, and some 200 KB per SM are in flight.
+// Otherwise the second reading is of the row again (from L2: a row is in use
+// by one cluster only).  A slot is written and read by one thread: no barrier.
+template <typename T, bool KEEP, bool GRAD, bool DENSE>
+__global__ void __launch_bounds__(kLossThreads, 6) loss_kernel(const LossArgs a) {
+  constexpr int VE = Vec<T>::VE;
+  __shared__ Sums shared[33];
+  extern __shared__ uint4 kept[];
+  const int rank = (int)(blockIdx.x % a.split);
+  const LossRow<T> r(a, blockIdx.x / a.split, threadIdx.x == 0 && rank == 0);
+  const float w = a.t.weights ? a.t.weights[r.row] : 1.f;
+  const bool idle = w == 0.f;  // a padded row: not read, loss and gradient 0
+  const int v0 = rank * a.vps;
+  const int n = min(a.vps, (r.shift + a.vocab + VE - 1) / VE - v0);  // the slice's vectors; below 1 past the row
+  const int first = v0 * VE - r.shift;                                // its first element (in the row or just before)
+  const int lo = max(0, first), hi = min(a.vocab, first + max(n, 0) * VE);
+
+  if (KEEP && !idle) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int e0 = first + i * VE;
+      const uint32_t in = rows::inside<VE>(e0, a.vocab);
+      if (in == rows::kFull<VE>) {
+        if (r.allowed(e0))
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(kept + i)),
+                       "l"(r.z + e0)
+                       : "memory");
+      } else {
+        kept[i] = rows::load_raw(r.z, e0, in, in);
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+  auto vector = [&](int i, int e0, uint32_t ok) {
+    return KEEP ? kept[i] : rows::load_raw(r.z, e0, rows::inside<VE>(e0, a.vocab), ok);
+  };
+
+  Sums v = nothing();
+  if (!idle) {
+    float2 sum = make_float2(0.f, 0.f);
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int e0 = first + i * VE;
+      const uint32_t ok = r.allowed(e0);
+      if (ok == 0) continue;
+      float x[VE];
+      Vec<T>::unpack(vector(i, e0, ok), x);
+      if (ok != rows::kFull<VE>) {
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+          if (!(ok >> j & 1)) x[j] = kNegInf;
+      }
+      const float m = top_of<VE>(x, kNegInf);
+      if (!(m <= v.m)) {  // a new maximum, or a NaN: what is summed so far relative to it
+        const float f = v.m == kNegInf ? 0.f : exp2_fast((v.m - m) * rows::kLog2e);
+        sum.x *= f;
+        sum.y *= f;
+        v.d = v.t != 0.f ? v.d + v.t * (m - v.m) : 0.f;
+        v.m = m;
+      }
+      if (DENSE) {
+        float t[VE];
+        r.targets(e0, ok, t);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+          v.t += t[j];
+          if (t[j] != 0.f && v.m != kNegInf) v.d += t[j] * (v.m - x[j]);
+        }
+      }
+      exps<VE>(x, v.m == kNegInf ? 0.f : v.m, &sum);  // -inf - -inf would be a NaN
+    }
+    v.s = sum.x + sum.y;
+    if (!DENSE) r.list_sums(lo, hi, rank == 0, v);
+  }
+  v = join_all(v, shared, a.split);
+  const bool none = idle || v.m == kNegInf;  // nothing is left of the row
+  if (rank == 0 && threadIdx.x == 0) {
+    if (a.loss) a.loss[r.row] = none ? 0.f : w * ((v.t != 0.f ? v.t * logf(v.s) : 0.f) + v.d);
+    if (a.stats) {
+      a.stats[3 * r.row] = none ? kNegInf : v.m;
+      a.stats[3 * r.row + 1] = v.s;
+      a.stats[3 * r.row + 2] = v.t;
+    }
+  }
+  if (GRAD) {
+    T* g = (T*)a.grad + r.row * a.grad_stride;
+    const bool whole = rows::lines_up(g, r.shift);
+    const float c = none || v.t == 0.f ? 0.f : w * v.t / v.s;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int e0 = first + i * VE;
+      const uint32_t ok = none ? 0 : r.allowed(e0);
+      float x[VE];
+      grad_vector<T, DENSE>(r, c != 0.f && ok ? vector(i, e0, ok) : make_uint4(0, 0, 0, 0), e0, ok, v.m, c, w, x);
+      rows::store<T, VE>(g, e0, rows::inside<VE>(e0, a.vocab), whole, x);
+    }
+    if (!DENSE && !none) {
+      __syncthreads();  // the listed tokens' elements again, now with their targets
+      r.list_grads(lo, hi, g, v.m, c, w);
+    }
+  }
+  cluster_done(a.split);
+}
+
+// The gradient from the sums of an earlier forward pass; the slices of a row
+// are independent CTAs.
+template <typename T, int NV, bool DENSE>
+__global__ void __launch_bounds__(kLossThreads) loss_bwd_kernel(const LossArgs a) {
+  constexpr int VE = Vec<T>::VE;
+  const int rank = (int)(blockIdx.x % a.split);
+  const LossRow<T> r(a, blockIdx.x / a.split, threadIdx.x == 0 && rank == 0);
+  float w = a.t.weights ? a.t.weights[r.row] : 1.f;
+  const float m = a.stats[3 * r.row], s = a.stats[3 * r.row + 1], mass = a.stats[3 * r.row + 2];
+  const bool none = w == 0.f || m == kNegInf;
+  if (a.upstream) w *= a.upstream[r.row];
+  const float c = none || mass == 0.f ? 0.f : w * mass / s;
+  const int v0 = rank * a.vps;
+  const int n = min(a.vps, (r.shift + a.vocab + VE - 1) / VE - v0);
+  const int first = v0 * VE - r.shift;
+  T* g = (T*)a.grad + r.row * a.grad_stride;
+  const bool whole = rows::lines_up(g, r.shift);
+  uint4 raw[NV];
+  uint32_t ok[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int k = i * blockDim.x + threadIdx.x, e0 = first + k * VE;
+    ok[i] = k < n && !none ? r.allowed(e0) : 0;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (ok[i] && c != 0.f) raw[i] = rows::load_raw(r.z, e0, rows::inside<VE>(e0, a.vocab), ok[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int k = i * blockDim.x + threadIdx.x, e0 = first + k * VE;
+    if (k >= n) break;
+    float x[VE];
+    grad_vector<T, DENSE>(r, raw[i], e0, ok[i], m, c, w, x);
+    rows::store<T, VE>(g, e0, rows::inside<VE>(e0, a.vocab), whole, x);
+  }
+  if (!DENSE && !none) {
+    __syncthreads();
+    r.list_grads(max(0, first), min(a.vocab, first + max(n, 0) * VE), g, m, c, w);
+  }
+}
+
+template <typename T, bool KEEP, bool GRAD, bool DENSE>
+int launch_loss(const LossArgs& a, int64_t n_rows, int threads, cudaStream_t s) {
+  if (n_rows * a.split > 0x7fffffff) return set_error(CNNUE_ERR_INVALID_ARG, "too many rows for one call");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(n_rows * a.split));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = KEEP ? (size_t)a.vps * 16 : 0;
+  cfg.stream = s;
+  if (cfg.dynamicSmemBytes > 47 * 1024)
+    CNNUE_CUDA_TRY(cudaFuncSetAttribute(loss_kernel<T, KEEP, GRAD, DENSE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)cfg.dynamicSmemBytes));
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {(unsigned)a.split, 1, 1};
+  cfg.attrs = &attr;
+  cfg.numAttrs = a.split > 1 ? 1 : 0;
+  CNNUE_CUDA_TRY(cudaLaunchKernelEx(&cfg, loss_kernel<T, KEEP, GRAD, DENSE>, a));
   return check_launch_error("loss_kernel");
+}
+
+// Vectors that cover a row: one more only where a row may start inside one.
+template <typename T>
+int64_t row_vectors(const void* p, int64_t stride, int64_t vocab) {
+  constexpr int VE = Vec<T>::VE;
+  return (uintptr_t)p % 16 == 0 && stride % VE == 0 ? (vocab + VE - 1) / VE : rows::max_vectors<T>(vocab);
+}
+
+constexpr int kMaxCluster = 8;      // the portable size
+constexpr int kSliceVectors = 2048;  // 32 KB of shared memory: 6 CTAs per SM
+constexpr int kMostVectors = 4096;   // 64 KB: 3 CTAs per SM
+
+template <typename T, bool GRAD>
+int run_loss(LossArgs a, int64_t n_rows, cudaStream_t s) {
+  const int64_t nv = row_vectors<T>(a.z, a.z_stride, a.vocab);
+  int64_t ctas = 1;
+  while (ctas < kMaxCluster && nv > kSliceVectors * ctas) ctas *= 2;
+  a.split = (int)ctas;
+  a.vps = (int)((nv + ctas - 1) / ctas);
+  const int threads = (int)std::min<int64_t>(kLossThreads, (a.vps + 127) / 128 * 32);  // 4 vectors per thread, or more
+  if (GRAD && a.vps <= kMostVectors)
+    return a.t.dense ? launch_loss<T, GRAD, GRAD, true>(a, n_rows, threads, s)
+                     : launch_loss<T, GRAD, GRAD, false>(a, n_rows, threads, s);
+  return a.t.dense ? launch_loss<T, false, GRAD, true>(a, n_rows, threads, s)
+                   : launch_loss<T, false, GRAD, false>(a, n_rows, threads, s);
+}
+
+template <typename T>
+int run_loss_bwd(LossArgs a, int64_t n_rows, cudaStream_t s) {
+  constexpr int NV = 4;
+  const int64_t nv = row_vectors<T>(a.z, a.z_stride, a.vocab);
+  a.vps = (int)std::min<int64_t>(nv, NV * kLossThreads);
+  a.split = (int)((nv + a.vps - 1) / a.vps);
+  const int threads = (int)std::min<int64_t>(kLossThreads, (a.vps + NV * 32 - 1) / (NV * 32) * 32);
+  if (n_rows * a.split > 0x7fffffff) return set_error(CNNUE_ERR_INVALID_ARG, "too many rows for one call");
+  if (a.t.dense)
+    loss_bwd_kernel<T, NV, true><<<(unsigned)(n_rows * a.split), threads, 0, s>>>(a);
+  else
+    loss_bwd_kernel<T, NV, false><<<(unsigned)(n_rows * a.split), threads, 0, s>>>(a);
+  return check_launch_error("loss_bwd_kernel");
 }
 
 template <bool FWD, bool GRAD>
 int pick_loss(const LossArgs& a, int type, int64_t n_rows, cudaStream_t s) {
-  if (type == CNNUE_F32) return launch_loss<float, FWD, GRAD>(a, n_rows, s);
-  if (type == CNNUE_BF16) return launch_loss<__nv_bfloat16, FWD, GRAD>(a, n_rows, s);
-  return launch_loss<__half, FWD, GRAD>(a, n_rows, s);
+  if (!FWD)
+    return type == CNNUE_F32    ? run_loss_bwd<float>(a, n_rows, s)
+           : type == CNNUE_BF16 ? run_loss_bwd<__nv_bfloat16>(a, n_rows, s)
+                                : run_loss_bwd<__half>(a, n_rows, s);
+  return type == CNNUE_F32    ? run_loss<float, GRAD>(a, n_rows, s)
+         : type == CNNUE_BF16 ? run_loss<__nv_bfloat16, GRAD>(a, n_rows, s)
+                              : run_loss<__half, GRAD>(a, n_rows, s);
 }
 
 // ---- argument checks --------------------------------------------------------
@@ -524,7 +770,7 @@ int cnnue_policy_loss_fwd(const void* d_logits, int64_t logits_stride, int logit
   if (vocab == 0) return set_error(CNNUE_ERR_INVALID_ARG, "empty vocabulary");
   if (int st = check_rows(d_logits, logits_stride, logits_type, n_rows, vocab, false, "logits")) return st;
   if (!d_loss || !d_stats) return set_error(CNNUE_ERR_INVALID_ARG, "null loss or stats");
-  const LossArgs a{d_logits, logits_stride, (int)vocab, *targets, nullptr, d_loss, d_stats, nullptr, 0, d_status};
+  const LossArgs a{d_logits, logits_stride, (int)vocab, 0, 0, *targets, nullptr, d_loss, d_stats, nullptr, 0, d_status};
   return pick_loss<true, false>(a, logits_type, n_rows, (cudaStream_t)stream);
 }
 
@@ -541,7 +787,7 @@ int cnnue_policy_loss_bwd(const void* d_logits, int64_t logits_stride, int logit
   const int b = element_bytes(logits_type);
   if (overlap(d_logits, logits_stride, b, d_grad, grad_stride, b, n_rows, vocab))
     return set_error(CNNUE_ERR_INVALID_ARG, "grad overlaps the logits");
-  const LossArgs a{d_logits,   logits_stride, (int)vocab, *targets,    d_upstream, nullptr, const_cast<float*>(d_stats),
+  const LossArgs a{d_logits,   logits_stride, (int)vocab, 0, 0, *targets, d_upstream, nullptr, const_cast<float*>(d_stats),
                    d_grad, grad_stride, d_status};
   return pick_loss<false, true>(a, logits_type, n_rows, (cudaStream_t)stream);
 }
@@ -559,7 +805,7 @@ int cnnue_policy_loss_grad(const void* d_logits, int64_t logits_stride, int logi
   const int b = element_bytes(logits_type);
   if (overlap(d_logits, logits_stride, b, d_grad, grad_stride, b, n_rows, vocab))
     return set_error(CNNUE_ERR_INVALID_ARG, "grad overlaps the logits");
-  const LossArgs a{d_logits, logits_stride, (int)vocab, *targets, nullptr, d_loss, nullptr, d_grad, grad_stride, d_status};
+  const LossArgs a{d_logits, logits_stride, (int)vocab, 0, 0, *targets, nullptr, d_loss, nullptr, d_grad, grad_stride, d_status};
   return pick_loss<true, true>(a, logits_type, n_rows, (cudaStream_t)stream);
 }
 

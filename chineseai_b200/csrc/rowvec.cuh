@@ -156,6 +156,18 @@ __device__ __forceinline__ void load(const T* row, int e0, uint32_t in, uint32_t
   }
 }
 
+// The raw vector e0 with at least the elements of `want` in it (the others are
+// whatever a whole load brings, or 0).
+template <typename T>
+__device__ __forceinline__ uint4 load_raw(const T* row, int e0, uint32_t in, uint32_t want) {
+  constexpr int VE = Vec<T>::VE;
+  if (in == kFull<VE>) return load16(row + e0);
+  float x[VE];
+#pragma unroll
+  for (int i = 0; i < VE; ++i) x[i] = want >> i & 1 ? Vec<T>::up(row[e0 + i]) : 0.f;
+  return Vec<T>::pack(x);
+}
+
 // x to the elements of vector e0 (of the input's vectors, VE of them) of an
 // output row of TO.  `whole`: that vector's output starts on a 16-byte
 // boundary; else, or at the row's edges, element by element.
@@ -186,10 +198,31 @@ __device__ __forceinline__ int token_at(const void* list, int64_t i, bool wide) 
   return t < 0 ? -1 : t > 0x7fffffff ? 0x7fffffff : (int)t;
 }
 
+// Two fp32 operations in one instruction, each rounded as its scalar form.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  asm("{.reg .b64 ra, rb, rc;\n\tmov.b64 ra, {%0, %1};\n\tmov.b64 rb, {%2, %3};\n\t"
+      "add.rn.f32x2 rc, ra, rb;\n\tmov.b64 {%0, %1}, rc;}"
+      : "+f"(a.x), "+f"(a.y)
+      : "f"(b.x), "f"(b.y));
+  return a;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  asm("{.reg .b64 ra, rb, rc;\n\tmov.b64 ra, {%0, %1};\n\tmov.b64 rb, {%2, %3};\n\t"
+      "mul.rn.f32x2 rc, ra, rb;\n\tmov.b64 {%0, %1}, rc;}"
+      : "+f"(a.x), "+f"(a.y)
+      : "f"(b.x), "f"(b.y));
+  return a;
+}
+
 // Maximum that keeps a NaN.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
