@@ -5,6 +5,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "rowvec.cuh"
 
@@ -246,14 +247,34 @@ __device__ __forceinline__ bool token_ok(const RowMask& m, int t) {
   return !m.dead && (!m.words || (__ldg(m.words + (t >> 5)) >> (t & 31) & 1));
 }
 
+// Exponentials are exp2(x c - B) with c = log2(e) in fp32 and B = m c rounded:
+// one fused operation per element before the instruction, and because every
+// thread and both passes take the same B for the same m, B's rounding cancels
+// in exp / sum; the loss takes it out (residual()).  |m| near fp32's limit,
+// where m c would overflow, goes through (x - m) c.
 struct Sums {
-  float m, s, t, d;  // maximum, sum of exp(z - m), target mass, sum of t (m - z)
+  float m, s, t, d;  // maximum, sum of exp2(z c - B(m)), target mass, sum of t (m - z)
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+__device__ __forceinline__ bool huge(float m) { return fabsf(m) > 1e38f; }  // infinities too
+__device__ __forceinline__ float base(float m) { return __fmul_rn(m, rows::kLog2e); }
+// exp2(z c - B(from)) times this is exp2(z c - B(to)); from -inf: 0.
+__device__ __forceinline__ float rebase(float from, float to) {
+  if (from == kNegInf) return 0.f;
+  return exp2_fast(huge(from) || huge(to) ? (from - to) * rows::kLog2e : base(from) - base(to));
+}
+// exp2(z c - B(m)) of one logit, m not -inf.
+__device__ __forceinline__ float exp_of(float z, float m) {
+  return exp2_fast(huge(m) ? (z - m) * rows::kLog2e : fmaf(z, rows::kLog2e, -base(m)));
+}
+// log of what B's rounding put into the sum.
+__device__ __forceinline__ float residual(float m) {
+  return huge(m) ? 0.f : 0.693147180559945309f * fmaf(m, rows::kLog2e, -base(m));
 }
 __device__ __forceinline__ float lane_sum(float x) {
 #pragma unroll
@@ -267,7 +288,7 @@ __device__ __forceinline__ Sums join_lanes(Sums v) {
   float m;
   asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v.m));
   if (m != kNegInf) {
-    v.s = v.m == kNegInf ? 0.f : v.s * exp2_fast((v.m - m) * rows::kLog2e);
+    v.s *= rebase(v.m, m);
     v.d = v.t != 0.f ? v.d + v.t * (m - v.m) : 0.f;
   }
   v.m = m;
@@ -321,7 +342,8 @@ struct LossRow {
     list = a.t.index ? (const char*)a.t.index + row * a.t.index_stride * a.t.index_bytes : nullptr;
     prob = a.t.prob ? a.t.prob + row * a.t.prob_stride : nullptr;
   }
-  __device__ __forceinline__ uint32_t allowed(int e0) const {
+  __device__ __forceinline__ uint32_t allowed(int e0, bool whole) const {
+    if (whole) return mask.dead ? 0 : mask.words ? rows::allowed_whole<VE>(mask.words, e0) : rows::kFull<VE>;
     return mask.dead ? 0 : mask.words ? rows::allowed<VE>(mask.words, e0, a.vocab) : rows::inside<VE>(e0, a.vocab);
   }
   // The dense targets of vector e0, 0 where `ok` has no bit.
@@ -385,35 +407,42 @@ struct LossRow {
       if (j < k) continue;  // an earlier entry's
       for (; j < a.t.count; ++j)
         if (rows::token_at(list, j, wide) == tok) t += mass(j);
-      g[tok] = Vec<T>::down((c == 0.f ? 0.f : c * exp2_fast((Vec<T>::up(z[tok]) - m) * rows::kLog2e)) - w * t);
+      g[tok] = Vec<T>::down((c == 0.f ? 0.f : c * exp_of(Vec<T>::up(z[tok]), m)) - w * t);
     }
   }
 };
 
-// exp(x - m) of a vector (m finite or NaN); *sum gets their sum.
+// exp2(x c - B(m)) of a vector, m not -inf; *sum gets their sum.
 template <int VE>
 __device__ __forceinline__ void exps(float* x, float m, float2* sum) {
-  const float2 minus = make_float2(-m, -m), scale = make_float2(rows::kLog2e, rows::kLog2e);
+  if (!huge(m)) {
+    const float2 c = make_float2(rows::kLog2e, rows::kLog2e), minus = make_float2(-base(m), -base(m));
 #pragma unroll
-  for (int j = 0; j < VE; j += 2) {
-    float2 d = rows::mul2(rows::add2(make_float2(x[j], x[j + 1]), minus), scale);
-    d.x = exp2_fast(d.x);
-    d.y = exp2_fast(d.y);
-    if (sum) *sum = rows::add2(*sum, d);
-    x[j] = d.x;
-    x[j + 1] = d.y;
+    for (int j = 0; j < VE; j += 2) {
+      const float2 d = rows::fma2(make_float2(x[j], x[j + 1]), c, minus);
+      x[j] = exp2_fast(d.x);
+      x[j + 1] = exp2_fast(d.y);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VE; ++j) x[j] = exp2_fast((x[j] - m) * rows::kLog2e);
+  }
+  if (sum) {
+#pragma unroll
+    for (int j = 0; j < VE; j += 2) *sum = rows::add2(*sum, make_float2(x[j], x[j + 1]));
   }
 }
 template <int VE>
-__device__ __forceinline__ float top_of(const float* x, float m) {
+__device__ __forceinline__ float top_of(const float* x) {
+  float m = rows::max_nan(x[0], x[1]);
 #pragma unroll
-  for (int j = 0; j < VE; j += 2) m = rows::max_nan(m, x[j], x[j + 1]);
+  for (int j = 2; j < VE; j += 2) m = rows::max_nan(m, x[j], x[j + 1]);
   return m;
 }
 
-// The gradient's vector e0 from the raw logits: c exp(z - m) - w t on `ok`, 0
-// elsewhere.  c = 0: nothing but the targets (and the logits are not looked
-// at, so no NaN comes from them).
+// The gradient's vector e0 from the raw logits: c exp2(z c' - B(m)) - w t on
+// `ok`, 0 elsewhere.  c = 0: nothing but the targets (and the logits are not
+// looked at, so no NaN comes from them).
 template <typename T, bool DENSE>
 __device__ __forceinline__ void grad_vector(const LossRow<T>& r, const uint4& raw, int e0, uint32_t ok, float m, float c,
                                             float w, float* x) {
@@ -446,6 +475,30 @@ __device__ __forceinline__ void grad_vector(const LossRow<T>& r, const uint4& ra
 
 constexpr int kLossThreads = 256;
 
+// A CTA's slice of a row: vectors 0 .. n - 1, vector i at element first + i VE.
+// All but the row's first and last are whole; whole ones are [from, to).
+template <int VE>
+struct Slice {
+  int first, n, from, to, lo, hi;
+  __device__ __forceinline__ Slice(int rank, int vps, int shift, int vocab) {
+    first = rank * vps * VE - shift;
+    n = max(0, min(vps, (shift + vocab + VE - 1) / VE - rank * vps));
+    from = n > 0 && first < 0 ? 1 : 0;
+    to = n > 0 && first + n * VE > vocab ? n - 1 : n;
+    lo = max(0, first);
+    hi = min(vocab, first + n * VE);
+  }
+  // f(vector, its first element, whether it is whole) for this thread's share,
+  // the same one at every call.
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll 2
+    for (int i = from + threadIdx.x; i < to; i += blockDim.x) f(i, first + i * VE, std::true_type{});
+    if (threadIdx.x == 0 && from == 1) f(0, first, std::false_type{});
+    if (threadIdx.x == 0 && to < n && (n > 1 || from == 0)) f(n - 1, first + (n - 1) * VE, std::false_type{});
+  }
+};
+
 // Loss, and with GRAD the gradient, of one slice of a row; the slices of a row
 // are the CTAs of a cluster.  A thread takes every blockDim-th vector of the
 // slice.  KEEP: it copies them into shared memory, all in flight at once, and
@@ -463,47 +516,38 @@ __global__ void __launch_bounds__(kLossThreads, 6) loss_kernel(const LossArgs a)
   const LossRow<T> r(a, blockIdx.x / a.split, threadIdx.x == 0 && rank == 0);
   const float w = a.t.weights ? a.t.weights[r.row] : 1.f;
   const bool idle = w == 0.f;  // a padded row: not read, loss and gradient 0
-  const int v0 = rank * a.vps;
-  const int n = min(a.vps, (r.shift + a.vocab + VE - 1) / VE - v0);  // the slice's vectors; below 1 past the row
-  const int first = v0 * VE - r.shift;                                // its first element (in the row or just before)
-  const int lo = max(0, first), hi = min(a.vocab, first + max(n, 0) * VE);
+  const Slice<VE> slice(rank, a.vps, r.shift, a.vocab);
 
   if (KEEP && !idle) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      const int e0 = first + i * VE;
-      const uint32_t in = rows::inside<VE>(e0, a.vocab);
-      if (in == rows::kFull<VE>) {
-        if (r.allowed(e0))
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(kept + i)),
-                       "l"(r.z + e0)
-                       : "memory");
-      } else {
-        kept[i] = rows::load_raw(r.z, e0, in, in);
-      }
-    }
+    slice.each([&](int i, int e0, auto whole) {
+      if (whole && r.allowed(e0, true))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(kept + i)),
+                     "l"(r.z + e0)
+                     : "memory");
+    });
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
-  auto vector = [&](int i, int e0, uint32_t ok) {
-    return KEEP ? kept[i] : rows::load_raw(r.z, e0, rows::inside<VE>(e0, a.vocab), ok);
+  auto vector = [&](int i, int e0, uint32_t ok, auto whole) {
+    if (KEEP && whole) return kept[i];
+    return rows::load_raw(r.z, e0, whole ? rows::kFull<VE> : rows::inside<VE>(e0, a.vocab), ok);
   };
 
   Sums v = nothing();
   if (!idle) {
     float2 sum = make_float2(0.f, 0.f);
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      const int e0 = first + i * VE;
-      const uint32_t ok = r.allowed(e0);
-      if (ok == 0) continue;
+    slice.each([&](int i, int e0, auto whole) {
+      const uint32_t ok = r.allowed(e0, whole);
+      if (ok == 0) return;
       float x[VE];
-      Vec<T>::unpack(vector(i, e0, ok), x);
+      Vec<T>::unpack(vector(i, e0, ok, whole), x);
       if (ok != rows::kFull<VE>) {
 #pragma unroll
         for (int j = 0; j < VE; ++j)
           if (!(ok >> j & 1)) x[j] = kNegInf;
       }
-      const float m = top_of<VE>(x, kNegInf);
+      const float m = top_of<VE>(x);
       if (!(m <= v.m)) {  // a new maximum, or a NaN: what is summed so far relative to it
-        const float f = v.m == kNegInf ? 0.f : exp2_fast((v.m - m) * rows::kLog2e);
+        const float f = rebase(v.m, m);
         sum.x *= f;
         sum.y *= f;
         v.d = v.t != 0.f ? v.d + v.t * (m - v.m) : 0.f;
@@ -519,14 +563,14 @@ __global__ void __launch_bounds__(kLossThreads, 6) loss_kernel(const LossArgs a)
         }
       }
       exps<VE>(x, v.m == kNegInf ? 0.f : v.m, &sum);  // -inf - -inf would be a NaN
-    }
+    });
     v.s = sum.x + sum.y;
-    if (!DENSE) r.list_sums(lo, hi, rank == 0, v);
+    if (!DENSE) r.list_sums(slice.lo, slice.hi, rank == 0, v);
   }
   v = join_all(v, shared, a.split);
   const bool none = idle || v.m == kNegInf;  // nothing is left of the row
   if (rank == 0 && threadIdx.x == 0) {
-    if (a.loss) a.loss[r.row] = none ? 0.f : w * ((v.t != 0.f ? v.t * logf(v.s) : 0.f) + v.d);
+    if (a.loss) a.loss[r.row] = none ? 0.f : w * ((v.t != 0.f ? v.t * (logf(v.s) - residual(v.m)) : 0.f) + v.d);
     if (a.stats) {
       a.stats[3 * r.row] = none ? kNegInf : v.m;
       a.stats[3 * r.row + 1] = v.s;
@@ -535,18 +579,17 @@ __global__ void __launch_bounds__(kLossThreads, 6) loss_kernel(const LossArgs a)
   }
   if (GRAD) {
     T* g = (T*)a.grad + r.row * a.grad_stride;
-    const bool whole = rows::lines_up(g, r.shift);
+    const bool lines_up = rows::lines_up(g, r.shift);
     const float c = none || v.t == 0.f ? 0.f : w * v.t / v.s;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      const int e0 = first + i * VE;
-      const uint32_t ok = none ? 0 : r.allowed(e0);
+    slice.each([&](int i, int e0, auto whole) {
+      const uint32_t ok = none ? 0 : r.allowed(e0, whole);
       float x[VE];
-      grad_vector<T, DENSE>(r, c != 0.f && ok ? vector(i, e0, ok) : make_uint4(0, 0, 0, 0), e0, ok, v.m, c, w, x);
-      rows::store<T, VE>(g, e0, rows::inside<VE>(e0, a.vocab), whole, x);
-    }
+      grad_vector<T, DENSE>(r, c != 0.f && ok ? vector(i, e0, ok, whole) : make_uint4(0, 0, 0, 0), e0, ok, v.m, c, w, x);
+      rows::store<T, VE>(g, e0, whole ? rows::kFull<VE> : rows::inside<VE>(e0, a.vocab), lines_up, x);
+    });
     if (!DENSE && !none) {
       __syncthreads();  // the listed tokens' elements again, now with their targets
-      r.list_grads(lo, hi, g, v.m, c, w);
+      r.list_grads(slice.lo, slice.hi, g, v.m, c, w);
     }
   }
   cluster_done(a.split);
@@ -554,7 +597,7 @@ __global__ void __launch_bounds__(kLossThreads, 6) loss_kernel(const LossArgs a)
 
 // The gradient from the sums of an earlier forward pass; the slices of a row
 // are independent CTAs.
-template <typename T, int NV, bool DENSE>
+template <typename T, bool DENSE>
 __global__ void __launch_bounds__(kLossThreads) loss_bwd_kernel(const LossArgs a) {
   constexpr int VE = Vec<T>::VE;
   const int rank = (int)(blockIdx.x % a.split);
@@ -564,31 +607,19 @@ __global__ void __launch_bounds__(kLossThreads) loss_bwd_kernel(const LossArgs a
   const bool none = w == 0.f || m == kNegInf;
   if (a.upstream) w *= a.upstream[r.row];
   const float c = none || mass == 0.f ? 0.f : w * mass / s;
-  const int v0 = rank * a.vps;
-  const int n = min(a.vps, (r.shift + a.vocab + VE - 1) / VE - v0);
-  const int first = v0 * VE - r.shift;
+  const Slice<VE> slice(rank, a.vps, r.shift, a.vocab);
   T* g = (T*)a.grad + r.row * a.grad_stride;
-  const bool whole = rows::lines_up(g, r.shift);
-  uint4 raw[NV];
-  uint32_t ok[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int k = i * blockDim.x + threadIdx.x, e0 = first + k * VE;
-    ok[i] = k < n && !none ? r.allowed(e0) : 0;
-    raw[i] = make_uint4(0, 0, 0, 0);
-    if (ok[i] && c != 0.f) raw[i] = rows::load_raw(r.z, e0, rows::inside<VE>(e0, a.vocab), ok[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int k = i * blockDim.x + threadIdx.x, e0 = first + k * VE;
-    if (k >= n) break;
+  const bool lines_up = rows::lines_up(g, r.shift);
+  slice.each([&](int i, int e0, auto whole) {
+    const uint32_t in = whole ? rows::kFull<VE> : rows::inside<VE>(e0, a.vocab);
+    const uint32_t ok = none ? 0 : r.allowed(e0, whole);
     float x[VE];
-    grad_vector<T, DENSE>(r, raw[i], e0, ok[i], m, c, w, x);
-    rows::store<T, VE>(g, e0, rows::inside<VE>(e0, a.vocab), whole, x);
-  }
+    grad_vector<T, DENSE>(r, c != 0.f && ok ? rows::load_raw(r.z, e0, in, ok) : make_uint4(0, 0, 0, 0), e0, ok, m, c, w, x);
+    rows::store<T, VE>(g, e0, in, lines_up, x);
+  });
   if (!DENSE && !none) {
     __syncthreads();
-    r.list_grads(max(0, first), min(a.vocab, first + max(n, 0) * VE), g, m, c, w);
+    r.list_grads(slice.lo, slice.hi, g, m, c, w);
   }
 }
 
@@ -647,9 +678,9 @@ int run_loss_bwd(LossArgs a, int64_t n_rows, cudaStream_t s) {
   const int threads = (int)std::min<int64_t>(kLossThreads, (a.vps + NV * 32 - 1) / (NV * 32) * 32);
   if (n_rows * a.split > 0x7fffffff) return set_error(CNNUE_ERR_INVALID_ARG, "too many rows for one call");
   if (a.t.dense)
-    loss_bwd_kernel<T, NV, true><<<(unsigned)(n_rows * a.split), threads, 0, s>>>(a);
+    loss_bwd_kernel<T, true><<<(unsigned)(n_rows * a.split), threads, 0, s>>>(a);
   else
-    loss_bwd_kernel<T, NV, false><<<(unsigned)(n_rows * a.split), threads, 0, s>>>(a);
+    loss_bwd_kernel<T, false><<<(unsigned)(n_rows * a.split), threads, 0, s>>>(a);
   return check_launch_error("loss_bwd_kernel");
 }
 

@@ -135,6 +135,15 @@ __device__ __forceinline__ uint4 load16(const void* p) {
   return r;
 }
 
+// allowed() for a vector that lies inside the row.
+template <int VE>
+__device__ __forceinline__ uint32_t allowed_whole(const uint32_t* __restrict__ mask, int e0) {
+  const int w = e0 >> 5, sh = e0 & 31;
+  uint32_t b = __ldg(mask + w) >> sh;
+  if (sh > 32 - VE) b |= __ldg(mask + w + 1) << (32 - sh);
+  return b & kFull<VE>;
+}
+
 // The elements of vector e0 that `want` names (a subset of inside()); the
 // others get `rest`.
 template <typename T>
@@ -211,6 +220,13 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
       "mul.rn.f32x2 rc, ra, rb;\n\tmov.b64 {%0, %1}, rc;}"
       : "+f"(a.x), "+f"(a.y)
       : "f"(b.x), "f"(b.y));
+  return a;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  asm("{.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%0, %1};\n\tmov.b64 rb, {%2, %3};\n\tmov.b64 rc, {%4, %5};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;}"
+      : "+f"(a.x), "+f"(a.y)
+      : "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return a;
 }
 
