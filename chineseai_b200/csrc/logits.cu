@@ -313,13 +313,30 @@ __device__ __forceinline__ Sums join_all(Sums v, Sums* shared, int ctas) {
     if (threadIdx.x == 0) shared[32] = v;
     cluster.sync();
     v = join_lanes(lane < ctas ? *cluster.map_shared_rank(shared + 32, lane) : nothing());
-    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    // nothing is handed over: it only keeps this CTA's shared memory until all have read it
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   }
   return v;
 }
 __device__ __forceinline__ void cluster_done(int ctas) {
   if (ctas > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
+
+// Which of a list's tokens may occur in it more than once: a token's bit (by
+// its low 13 bits) is set a second time.  Tokens that share a bit by chance
+// are marked too, which costs time, not results.
+struct Repeats {
+  static constexpr int kWords = 256;
+  uint32_t once[kWords], more[kWords];
+  __device__ __forceinline__ void clear() {
+    for (int i = threadIdx.x; i < kWords; i += blockDim.x) once[i] = more[i] = 0;
+  }
+  __device__ __forceinline__ void mark(int tok) {
+    const uint32_t word = (uint32_t)tok / 32 % kWords, bit = 1u << (tok & 31);
+    if (atomicOr(once + word, bit) & bit) atomicOr(more + word, bit);
+  }
+  __device__ __forceinline__ bool marked(int tok) const { return more[(uint32_t)tok / 32 % kWords] >> (tok & 31) & 1; }
+};
 
 // One row's tensors as a CTA sees them.
 template <typename T>
@@ -376,12 +393,14 @@ struct LossRow {
   }
   __device__ __forceinline__ float mass(int64_t k) const { return prob ? __ldg(prob + k) : 1.f; }
 
-  // Mass and d of the list's entries on tokens [lo, hi), relative to m.
-  __device__ __forceinline__ void list_sums(int lo, int hi, bool tell, Sums& v) const {
+  // Mass and d of the list's entries on tokens [lo, hi), relative to v.m;
+  // repeated tokens are marked.
+  __device__ __forceinline__ void list_sums(int lo, int hi, bool tell, Sums& v, Repeats& repeats) const {
     for (int64_t k = threadIdx.x; k < a.t.count; k += blockDim.x) {
       if (tell && rows::token_at(list, k, wide) >= a.vocab) atomicOr(a.status, CNNUE_STATUS_BAD_INDEX);
       const int tok = entry(k);
       if (tok < lo || tok >= hi) continue;
+      if (a.t.count > 1) repeats.mark(tok);
       const float t = mass(k);
       if (t == 0.f) continue;
       const float x = Vec<T>::up(z[tok]);
@@ -395,18 +414,27 @@ struct LossRow {
     }
   }
 
-  // The gradient at the listed tokens [lo, hi): c exp(z - m) - w t, with t
-  // summed in list order by the thread of the token's first entry.
-  __device__ __forceinline__ void list_grads(int lo, int hi, T* g, float m, float c, float w) const {
+  // The gradient at the listed tokens [lo, hi): c exp(z - m) - w t.  A token
+  // that may be listed more than once is summed in list order by the thread of
+  // its first entry (every thread walks the whole list, so that a warp's lanes
+  // stay together).
+  __device__ __forceinline__ void list_grads(int lo, int hi, T* g, float m, float c, float w, const Repeats& repeats) const {
     for (int64_t k = threadIdx.x; k < a.t.count; k += blockDim.x) {
       const int tok = entry(k);
       if (tok < lo || tok >= hi) continue;
-      float t = 0.f;
-      int64_t j = 0;
-      while (j < k && rows::token_at(list, j, wide) != tok) ++j;
-      if (j < k) continue;  // an earlier entry's
-      for (; j < a.t.count; ++j)
-        if (rows::token_at(list, j, wide) == tok) t += mass(j);
+      float t;
+      if (a.t.count == 1 || !repeats.marked(tok)) {
+        t = mass(k);
+      } else {
+        t = 0.f;
+        bool earlier = false;
+        for (int64_t j = 0; j < a.t.count; ++j) {
+          if (rows::token_at(list, j, wide) != tok) continue;
+          earlier |= j < k;
+          t += mass(j);
+        }
+        if (earlier) continue;
+      }
       g[tok] = Vec<T>::down((c == 0.f ? 0.f : c * exp_of(Vec<T>::up(z[tok]), m)) - w * t);
     }
   }
@@ -517,6 +545,9 @@ __global__ void __launch_bounds__(kLossThreads, 6) loss_kernel(const LossArgs a)
   const float w = a.t.weights ? a.t.weights[r.row] : 1.f;
   const bool idle = w == 0.f;  // a padded row: not read, loss and gradient 0
   const Slice<VE> slice(rank, a.vps, r.shift, a.vocab);
+  __shared__ Repeats repeats;
+  const bool lists = !DENSE && a.t.count > 1;
+  if (lists) repeats.clear();
 
   if (KEEP && !idle) {
     slice.each([&](int i, int e0, auto whole) {
@@ -565,7 +596,8 @@ __global__ void __launch_bounds__(kLossThreads, 6) loss_kernel(const LossArgs a)
       exps<VE>(x, v.m == kNegInf ? 0.f : v.m, &sum);  // -inf - -inf would be a NaN
     });
     v.s = sum.x + sum.y;
-    if (!DENSE) r.list_sums(slice.lo, slice.hi, rank == 0, v);
+    if (lists) __syncthreads();  // cleared
+    if (!DENSE) r.list_sums(slice.lo, slice.hi, rank == 0, v, repeats);
   }
   v = join_all(v, shared, a.split);
   const bool none = idle || v.m == kNegInf;  // nothing is left of the row
@@ -589,7 +621,7 @@ __global__ void __launch_bounds__(kLossThreads, 6) loss_kernel(const LossArgs a)
     });
     if (!DENSE && !none) {
       __syncthreads();  // the listed tokens' elements again, now with their targets
-      r.list_grads(slice.lo, slice.hi, g, v.m, c, w);
+      r.list_grads(slice.lo, slice.hi, g, v.m, c, w, repeats);
     }
   }
   cluster_done(a.split);
@@ -608,6 +640,15 @@ __global__ void __launch_bounds__(kLossThreads) loss_bwd_kernel(const LossArgs a
   if (a.upstream) w *= a.upstream[r.row];
   const float c = none || mass == 0.f ? 0.f : w * mass / s;
   const Slice<VE> slice(rank, a.vps, r.shift, a.vocab);
+  __shared__ Repeats repeats;
+  if (!DENSE && !none && a.t.count > 1) {
+    repeats.clear();
+    __syncthreads();
+    for (int64_t k = threadIdx.x; k < a.t.count; k += blockDim.x) {
+      const int tok = r.entry(k);
+      if (tok >= slice.lo && tok < slice.hi) repeats.mark(tok);
+    }
+  }
   T* g = (T*)a.grad + r.row * a.grad_stride;
   const bool lines_up = rows::lines_up(g, r.shift);
   slice.each([&](int i, int e0, auto whole) {
@@ -619,7 +660,7 @@ __global__ void __launch_bounds__(kLossThreads) loss_bwd_kernel(const LossArgs a
   });
   if (!DENSE && !none) {
     __syncthreads();
-    r.list_grads(slice.lo, slice.hi, g, m, c, w);
+    r.list_grads(slice.lo, slice.hi, g, m, c, w, repeats);
   }
 }
 
