@@ -276,43 +276,51 @@ __device__ __forceinline__ float exp_of(float z, float m) {
 __device__ __forceinline__ float residual(float m) {
   return huge(m) ? 0.f : 0.693147180559945309f * fmaf(m, rows::kLog2e, -base(m));
 }
-__device__ __forceinline__ float lane_sum(float x) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
-  return x;
-}
-// The sums of 32 lanes, each relative to its own maximum, as one; every lane
-// gets the same bits.  A side without a logit above -inf has s = 0; mass that
-// sits on its -inf logits makes d infinite, as t (m - z) says.
+// The sums of N lanes (each group of N apart), each relative to its own
+// maximum, as one; every lane of a group gets the same bits.  A side without a
+// logit above -inf has s = 0; mass that sits on its -inf logits makes d
+// infinite, as t (m - z) says.
+template <int N>
 __device__ __forceinline__ Sums join_lanes(Sums v) {
-  float m;
-  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v.m));
+  float m = v.m;
+  if (N == 32) {
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v.m));
+  } else {
+#pragma unroll
+    for (int o = N / 2; o; o >>= 1) m = rows::max_nan(m, __shfl_xor_sync(~0u, m, o));
+  }
   if (m != kNegInf) {
     v.s *= rebase(v.m, m);
     v.d = v.t != 0.f ? v.d + v.t * (m - v.m) : 0.f;
   }
   v.m = m;
-  v.s = lane_sum(v.s);
-  v.t = lane_sum(v.t);
-  v.d = lane_sum(v.d);
+#pragma unroll
+  for (int o = N / 2; o; o >>= 1) {
+    v.s += __shfl_xor_sync(~0u, v.s, o);
+    v.t += __shfl_xor_sync(~0u, v.t, o);
+    v.d += __shfl_xor_sync(~0u, v.d, o);
+  }
   return v;
 }
 __device__ __forceinline__ Sums nothing() { return {kNegInf, 0.f, 0.f, 0.f}; }
 
+constexpr int kLossThreads = 256;  // at most 8 warps
+constexpr int kMaxCluster = 8;     // the portable size
+
 // The sums of the CTA's threads; then of the CTAs of its cluster, whose
-// `shared[32]` every CTA reads over distributed shared memory.  The caller
+// `shared[8]` every CTA reads over distributed shared memory.  The caller
 // waits for the cluster (cluster_done) before it leaves.
 __device__ __forceinline__ Sums join_all(Sums v, Sums* shared, int ctas) {
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  v = join_lanes(v);
+  v = join_lanes<32>(v);
   if (lane == 0) shared[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = join_lanes(lane < warps ? shared[lane] : nothing());
+  if (warps > 1) v = join_lanes<8>((lane & 7) < warps ? shared[lane & 7] : nothing());
   if (ctas > 1) {
     cg::cluster_group cluster = cg::this_cluster();
-    if (threadIdx.x == 0) shared[32] = v;
+    if (threadIdx.x == 0) shared[8] = v;
     cluster.sync();
-    v = join_lanes(lane < ctas ? *cluster.map_shared_rank(shared + 32, lane) : nothing());
+    v = join_lanes<8>((lane & 7) < ctas ? *cluster.map_shared_rank(shared + 8, lane & 7) : nothing());
     // nothing is handed over: it only keeps this CTA's shared memory until all have read it
     asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   }
@@ -393,6 +401,9 @@ struct LossRow {
   }
   __device__ __forceinline__ float mass(int64_t k) const { return prob ? __ldg(prob + k) : 1.f; }
 
+  template <bool DENSE>
+  __device__ void edge_grad(int e0, bool none, T* g, float m, float c, float w) const;
+
   // Mass and d of the list's entries on tokens [lo, hi), relative to v.m;
   // repeated tokens are marked.
   __device__ __forceinline__ void list_sums(int lo, int hi, bool tell, Sums& v, Repeats& repeats) const {
@@ -460,14 +471,6 @@ __device__ __forceinline__ void exps(float* x, float m, float2* sum) {
     for (int j = 0; j < VE; j += 2) *sum = rows::add2(*sum, make_float2(x[j], x[j + 1]));
   }
 }
-template <int VE>
-__device__ __forceinline__ float top_of(const float* x) {
-  float m = rows::max_nan(x[0], x[1]);
-#pragma unroll
-  for (int j = 2; j < VE; j += 2) m = rows::max_nan(m, x[j], x[j + 1]);
-  return m;
-}
-
 // The gradient's vector e0 from the raw logits: c exp2(z c' - B(m)) - w t on
 // `ok`, 0 elsewhere.  c = 0: nothing but the targets (and the logits are not
 // looked at, so no NaN comes from them).
@@ -501,7 +504,17 @@ __device__ __forceinline__ void grad_vector(const LossRow<T>& r, const uint4& ra
   }
 }
 
-constexpr int kLossThreads = 256;
+// The gradient of a row's partial vector.
+template <typename T>
+template <bool DENSE>
+__device__ __forceinline__ void LossRow<T>::edge_grad(int e0, bool none, T* g, float m, float c, float w) const {
+  const uint32_t in = rows::inside<VE>(e0, a.vocab), ok = none ? 0 : allowed(e0, false);
+  uint4 raw = make_uint4(0, 0, 0, 0);
+  if (c != 0.f && ok) raw = rows::load_raw(z, e0, in, ok);
+  float x[VE];
+  grad_vector<T, DENSE>(*this, raw, e0, ok, m, c, w, x);
+  rows::store<T, VE>(g, e0, in, false, x);
+}
 
 // A CTA's slice of a row: vectors 0 .. n - 1, vector i at element first + i VE.
 // All but the row's first and last are whole; whole ones are [from, to).
@@ -516,14 +529,19 @@ struct Slice {
     lo = max(0, first);
     hi = min(vocab, first + n * VE);
   }
-  // f(vector, its first element, whether it is whole) for this thread's share,
-  // the same one at every call.
-  template <typename F>
+  // f(i, e0, count) for this thread's share of the whole vectors: `count` (up
+  // to N) of them, i + j blockDim at e0 + j blockDim VE.  The same share at
+  // every call.
+  template <int N, typename F>
   __device__ __forceinline__ void each(F&& f) const {
-#pragma unroll 2
-    for (int i = from + threadIdx.x; i < to; i += blockDim.x) f(i, first + i * VE, std::true_type{});
-    if (threadIdx.x == 0 && from == 1) f(0, first, std::false_type{});
-    if (threadIdx.x == 0 && to < n && (n > 1 || from == 0)) f(n - 1, first + (n - 1) * VE, std::false_type{});
+    for (int i = from + threadIdx.x; i < to; i += N * blockDim.x)
+      f(i, first + i * VE, min(N, (to - i + (int)blockDim.x - 1) / (int)blockDim.x));
+  }
+  // f(first element) for the partial vectors, by two threads.
+  template <typename F>
+  __device__ __forceinline__ void edges(F&& f) const {
+    if (threadIdx.x == 0 && from == 1) f(first);
+    if (threadIdx.x == blockDim.x - 1 && to < n && (n > 1 || from == 0)) f(first + (n - 1) * VE);
   }
 };
 
@@ -531,17 +549,19 @@ struct Slice {
 // are the CTAs of a cluster.  A thread takes every blockDim-th vector of the
 // slice.  KEEP: it copies them into shared memory, all in flight at once, and
 // reads them there twice: for the row's sums (online, relative to the thread's
-// running maximum) and, once the cluster has joined those, for the gradient;
-// the row is read from memory once, and some 200 KB per SM are in flight.
-// Otherwise the second reading is of the row again (from L2: a row is in use
-// by one cluster only).  A slot is written and read by one thread: no barrier.
+// running maximum, kAhead vectors at a time) and, once the cluster has joined
+// those, for the gradient; the row is read from memory once, and some 200 KB
+// per SM are in flight.  Otherwise the second reading is of the row again
+// (from L2: a row is in use by one cluster only).  A slot is written and read
+// by one thread: no barrier.
+constexpr int kAhead = 4;
 template <typename T, bool KEEP, bool GRAD, bool DENSE>
-__global__ void __launch_bounds__(kLossThreads, 6) loss_kernel(const LossArgs a) {
+__global__ void __launch_bounds__(kLossThreads, DENSE ? 4 : 6) loss_kernel(const LossArgs a) {
   constexpr int VE = Vec<T>::VE;
-  __shared__ Sums shared[33];
+  __shared__ Sums shared[kLossThreads / 32 + 1];
   extern __shared__ uint4 kept[];
-  const int rank = (int)(blockIdx.x % a.split);
-  const LossRow<T> r(a, blockIdx.x / a.split, threadIdx.x == 0 && rank == 0);
+  const int rank = (int)(blockIdx.x & (a.split - 1));  // split: a power of two
+  const LossRow<T> r(a, blockIdx.x >> (31 - __clz(a.split)), threadIdx.x == 0 && rank == 0);
   const float w = a.t.weights ? a.t.weights[r.row] : 1.f;
   const bool idle = w == 0.f;  // a padded row: not read, loss and gradient 0
   const Slice<VE> slice(rank, a.vps, r.shift, a.vocab);
@@ -549,34 +569,26 @@ __global__ void __launch_bounds__(kLossThreads, 6) loss_kernel(const LossArgs a)
   const bool lists = !DENSE && a.t.count > 1;
   if (lists) repeats.clear();
 
+  const int stride = blockDim.x;
   if (KEEP && !idle) {
-    slice.each([&](int i, int e0, auto whole) {
-      if (whole && r.allowed(e0, true))
+    slice.template each<1>([&](int i, int e0, int) {
+      if (r.allowed(e0, true))
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(kept + i)),
                      "l"(r.z + e0)
                      : "memory");
     });
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
-  auto vector = [&](int i, int e0, uint32_t ok, auto whole) {
-    if (KEEP && whole) return kept[i];
-    return rows::load_raw(r.z, e0, whole ? rows::kFull<VE> : rows::inside<VE>(e0, a.vocab), ok);
-  };
 
   Sums v = nothing();
   if (!idle) {
     float2 sum = make_float2(0.f, 0.f);
-    slice.each([&](int i, int e0, auto whole) {
-      const uint32_t ok = r.allowed(e0, whole);
-      if (ok == 0) return;
-      float x[VE];
-      Vec<T>::unpack(vector(i, e0, ok, whole), x);
-      if (ok != rows::kFull<VE>) {
+    // raw[N] with -inf where nothing is allowed, ok[N]: the vectors at e0 + j stride VE
+    auto add = [&](const uint4* raw, const uint32_t* ok, int e0, auto n) {
+      constexpr int N = decltype(n)::value;
+      float m = Vec<T>::top(raw[0]);
 #pragma unroll
-        for (int j = 0; j < VE; ++j)
-          if (!(ok >> j & 1)) x[j] = kNegInf;
-      }
-      const float m = top_of<VE>(x);
+      for (int j = 1; j < N; ++j) m = rows::max_nan(m, Vec<T>::top(raw[j]));
       if (!(m <= v.m)) {  // a new maximum, or a NaN: what is summed so far relative to it
         const float f = rebase(v.m, m);
         sum.x *= f;
@@ -584,16 +596,41 @@ __global__ void __launch_bounds__(kLossThreads, 6) loss_kernel(const LossArgs a)
         v.d = v.t != 0.f ? v.d + v.t * (m - v.m) : 0.f;
         v.m = m;
       }
-      if (DENSE) {
-        float t[VE];
-        r.targets(e0, ok, t);
+      const float from = v.m == kNegInf ? 0.f : v.m;  // -inf - -inf would be a NaN
 #pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          v.t += t[j];
-          if (t[j] != 0.f && v.m != kNegInf) v.d += t[j] * (v.m - x[j]);
+      for (int j = 0; j < N; ++j) {
+        float x[VE];
+        Vec<T>::unpack(raw[j], x);
+        if (DENSE && ok[j]) {
+          float t[VE];
+          r.targets(e0 + j * stride * VE, ok[j], t);
+#pragma unroll
+          for (int k = 0; k < VE; ++k) {
+            v.t += t[k];
+            if (t[k] != 0.f && v.m != kNegInf) v.d += t[k] * (v.m - x[k]);
+          }
         }
+        exps<VE>(x, from, &sum);
       }
-      exps<VE>(x, v.m == kNegInf ? 0.f : v.m, &sum);  // -inf - -inf would be a NaN
+    };
+    slice.template each<kAhead>([&](int i, int e0, int count) {
+      uint4 raw[kAhead];
+      uint32_t ok[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        ok[j] = j < count ? r.allowed(e0 + j * stride * VE, true) : 0;
+        raw[j] = make_uint4(0, 0, 0, 0);
+        if (ok[j]) raw[j] = KEEP ? kept[i + j * stride] : rows::load16(r.z + e0 + j * stride * VE);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (ok[j] != rows::kFull<VE>) raw[j] = Vec<T>::only(raw[j], ok[j]);
+      add(raw, ok, e0, std::integral_constant<int, kAhead>{});
+    });
+    slice.edges([&](int e0) {
+      const uint32_t in = rows::inside<VE>(e0, a.vocab), ok = r.allowed(e0, false);
+      const uint4 raw = Vec<T>::only(rows::load_raw(r.z, e0, in, ok), ok);
+      add(&raw, &ok, e0, std::integral_constant<int, 1>{});
     });
     v.s = sum.x + sum.y;
     if (lists) __syncthreads();  // cleared
@@ -612,13 +649,32 @@ __global__ void __launch_bounds__(kLossThreads, 6) loss_kernel(const LossArgs a)
   if (GRAD) {
     T* g = (T*)a.grad + r.row * a.grad_stride;
     const bool lines_up = rows::lines_up(g, r.shift);
-    const float c = none || v.t == 0.f ? 0.f : w * v.t / v.s;
-    slice.each([&](int i, int e0, auto whole) {
-      const uint32_t ok = none ? 0 : r.allowed(e0, whole);
-      float x[VE];
-      grad_vector<T, DENSE>(r, c != 0.f && ok ? vector(i, e0, ok, whole) : make_uint4(0, 0, 0, 0), e0, ok, v.m, c, w, x);
-      rows::store<T, VE>(g, e0, whole ? rows::kFull<VE> : rows::inside<VE>(e0, a.vocab), lines_up, x);
-    });
+    const float c = none || v.t == 0.f ? 0.f : __fdividef(w * v.t, v.s);
+    if (!DENSE && KEEP && c != 0.f && !a.t.mask && !huge(v.m) && lines_up) {  // nothing to look out for
+      const float2 scale = make_float2(rows::kLog2e, rows::kLog2e), minus = make_float2(-base(v.m), -base(v.m));
+      const float2 cc = make_float2(c, c);
+      slice.template each<1>([&](int i, int e0, int) {
+        float x[VE];
+        Vec<T>::unpack(kept[i], x);
+#pragma unroll
+        for (int j = 0; j < VE; j += 2) {
+          float2 d = rows::fma2(make_float2(x[j], x[j + 1]), scale, minus);
+          d = rows::mul2(make_float2(exp2_fast(d.x), exp2_fast(d.y)), cc);
+          x[j] = d.x, x[j + 1] = d.y;
+        }
+        *reinterpret_cast<uint4*>(g + e0) = Vec<T>::pack(x);
+      });
+    } else {
+      slice.template each<1>([&](int i, int e0, int) {
+        const uint32_t ok = none ? 0 : r.allowed(e0, true);
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (c != 0.f && ok) raw = KEEP ? kept[i] : rows::load16(r.z + e0);
+        float x[VE];
+        grad_vector<T, DENSE>(r, raw, e0, ok, v.m, c, w, x);
+        rows::store<T, VE>(g, e0, rows::kFull<VE>, lines_up, x);
+      });
+    }
+    slice.edges([&](int e0) { r.template edge_grad<DENSE>(e0, none, g, v.m, c, w); });
     if (!DENSE && !none) {
       __syncthreads();  // the listed tokens' elements again, now with their targets
       r.list_grads(slice.lo, slice.hi, g, v.m, c, w, repeats);
@@ -651,13 +707,26 @@ __global__ void __launch_bounds__(kLossThreads) loss_bwd_kernel(const LossArgs a
   }
   T* g = (T*)a.grad + r.row * a.grad_stride;
   const bool lines_up = rows::lines_up(g, r.shift);
-  slice.each([&](int i, int e0, auto whole) {
-    const uint32_t in = whole ? rows::kFull<VE> : rows::inside<VE>(e0, a.vocab);
-    const uint32_t ok = none ? 0 : r.allowed(e0, whole);
-    float x[VE];
-    grad_vector<T, DENSE>(r, c != 0.f && ok ? rows::load_raw(r.z, e0, in, ok) : make_uint4(0, 0, 0, 0), e0, ok, m, c, w, x);
-    rows::store<T, VE>(g, e0, in, lines_up, x);
+  slice.template each<kAhead>([&](int, int e0, int count) {
+    uint4 raw[kAhead];
+    uint32_t ok[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int e = e0 + j * (int)blockDim.x * VE;
+      ok[j] = j < count && !none ? r.allowed(e, true) : 0;
+      raw[j] = make_uint4(0, 0, 0, 0);
+      if (c != 0.f && ok[j]) raw[j] = rows::load16(r.z + e);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (j >= count) break;
+      const int e = e0 + j * (int)blockDim.x * VE;
+      float x[VE];
+      grad_vector<T, DENSE>(r, raw[j], e, ok[j], m, c, w, x);
+      rows::store<T, VE>(g, e, rows::kFull<VE>, lines_up, x);
+    }
   });
+  slice.edges([&](int e0) { r.template edge_grad<DENSE>(e0, none, g, m, c, w); });
   if (!DENSE && !none) {
     __syncthreads();
     r.list_grads(slice.lo, slice.hi, g, m, c, w, repeats);
@@ -691,7 +760,6 @@ int64_t row_vectors(const void* p, int64_t stride, int64_t vocab) {
   return (uintptr_t)p % 16 == 0 && stride % VE == 0 ? (vocab + VE - 1) / VE : rows::max_vectors<T>(vocab);
 }
 
-constexpr int kMaxCluster = 8;      // the portable size
 constexpr int kSliceVectors = 2048;  // 32 KB of shared memory: 6 CTAs per SM
 constexpr int kMostVectors = 4096;   // 64 KB: 3 CTAs per SM
 

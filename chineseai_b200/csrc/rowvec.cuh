@@ -19,6 +19,18 @@ namespace rows {
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// Maximum that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // Element count of 16 bytes, and the conversions of one element and one vector.
 template <typename T>
 struct Vec;
@@ -34,7 +46,22 @@ struct Vec<float> {
   static __device__ __forceinline__ uint4 pack(const float* x) {
     return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
   }
+  // -inf where `ok` has no bit.
+  static __device__ __forceinline__ uint4 only(uint4 r, uint32_t ok) {
+    return make_uint4(ok & 1 ? r.x : 0xff800000u, ok & 2 ? r.y : 0xff800000u, ok & 4 ? r.z : 0xff800000u,
+                      ok & 8 ? r.w : 0xff800000u);
+  }
+  // The largest element; a NaN if there is one.
+  static __device__ __forceinline__ float top(const uint4& r) {
+    return max_nan(max_nan(__uint_as_float(r.x), __uint_as_float(r.y), __uint_as_float(r.z)), __uint_as_float(r.w));
+  }
 };
+
+// Word i of a 16-bit vector with `low` in the halves that `ok` does not name.
+__device__ __forceinline__ uint32_t only_word(uint32_t w, uint32_t ok, int i, uint32_t low) {
+  const uint32_t keep = (ok >> 2 * i & 1 ? 0x0000ffffu : 0u) | (ok >> 2 * i & 2 ? 0xffff0000u : 0u);
+  return (w & keep) | (low & ~keep);
+}
 
 template <>
 struct Vec<__nv_bfloat16> {
@@ -57,6 +84,16 @@ struct Vec<__nv_bfloat16> {
       memcpy(&w[i], &h, 4);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ uint4 only(const uint4& r, uint32_t ok) {
+    return make_uint4(only_word(r.x, ok, 0, 0xff80ff80u), only_word(r.y, ok, 1, 0xff80ff80u),
+                      only_word(r.z, ok, 2, 0xff80ff80u), only_word(r.w, ok, 3, 0xff80ff80u));
+  }
+  static __device__ __forceinline__ float top(const uint4& r) {
+    __nv_bfloat162 a, b, c, d;
+    memcpy(&a, &r.x, 4), memcpy(&b, &r.y, 4), memcpy(&c, &r.z, 4), memcpy(&d, &r.w, 4);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(a, b), __hmax2_nan(c, d));
+    return max_nan(__bfloat162float(m.x), __bfloat162float(m.y));
   }
 };
 
@@ -84,6 +121,16 @@ struct Vec<__half> {
       memcpy(&w[i], &h, 4);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ uint4 only(const uint4& r, uint32_t ok) {
+    return make_uint4(only_word(r.x, ok, 0, 0xfc00fc00u), only_word(r.y, ok, 1, 0xfc00fc00u),
+                      only_word(r.z, ok, 2, 0xfc00fc00u), only_word(r.w, ok, 3, 0xfc00fc00u));
+  }
+  static __device__ __forceinline__ float top(const uint4& r) {
+    __half2 a, b, c, d;
+    memcpy(&a, &r.x, 4), memcpy(&b, &r.y, 4), memcpy(&c, &r.z, 4), memcpy(&d, &r.w, 4);
+    const __half2 m = __hmax2_nan(__hmax2_nan(a, b), __hmax2_nan(c, d));
+    return max_nan(__half2float(m.x), __half2float(m.y));
   }
 };
 
@@ -228,18 +275,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "+f"(a.x), "+f"(a.y)
       : "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return a;
-}
-
-// Maximum that keeps a NaN.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
 }
 
 }  // namespace rows
