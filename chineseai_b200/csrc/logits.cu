@@ -20,6 +20,83 @@ using rows::Vec;
 constexpr int64_t kMaxVocab = (int64_t)1 << 30;  // element offsets inside a row are 32-bit
 
 // ---------------------------------------------------------------------------
+// What both operators share: a row's mask, a CTA's slice of a row, and the
+// tokens that a list may name more than once.
+// ---------------------------------------------------------------------------
+
+struct RowMask {
+  const uint32_t* words;  // null: everything is allowed (unless dead)
+  bool dead;
+};
+template <typename Rules>  // cnnue_logit_rules or cnnue_loss_targets
+__device__ __forceinline__ RowMask row_mask(const Rules& t, int64_t row, uint32_t* status, bool tell) {
+  RowMask m{nullptr, false};
+  if (!t.mask) return m;
+  const int64_t i = t.mask_index ? (int64_t)t.mask_index[row] : t.mask_rows == 1 ? 0 : row;
+  if (i >= t.mask_rows) {
+    m.dead = true;
+    if (tell) atomicOr(status, CNNUE_STATUS_BAD_INDEX);
+  } else if (i >= 0) {
+    m.words = t.mask + i * t.mask_stride;
+  }
+  return m;
+}
+__device__ __forceinline__ bool token_ok(const RowMask& m, int t) {
+  return !m.dead && (!m.words || (__ldg(m.words + (t >> 5)) >> (t & 31) & 1));
+}
+
+// A CTA's slice of a row: vectors 0 .. n - 1, vector i at element first + i VE.
+// All but the row's first and last are whole; whole ones are [from, to).
+template <int VE>
+struct Slice {
+  int first, n, from, to, lo, hi;
+  __device__ __forceinline__ Slice(int rank, int vps, int shift, int vocab) {
+    first = rank * vps * VE - shift;
+    n = max(0, min(vps, (shift + vocab + VE - 1) / VE - rank * vps));
+    from = n > 0 && first < 0 ? 1 : 0;
+    to = n > 0 && first + n * VE > vocab ? n - 1 : n;
+    lo = max(0, first);
+    hi = min(vocab, first + n * VE);
+  }
+  // f(i, e0, n) for this thread's share of the whole vectors, n = N (the
+  // vectors i + j blockDim, at e0 + j blockDim VE) and 1 for what is left.  The
+  // same share at every call.
+  template <int N, typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    const int stride = blockDim.x;
+    int i = from + threadIdx.x;
+    for (; i + (N - 1) * stride < to; i += N * stride) f(i, first + i * VE, std::integral_constant<int, N>{});
+    if (N > 1) {
+#pragma unroll 1
+      for (; i < to; i += stride) f(i, first + i * VE, std::integral_constant<int, 1>{});
+    }
+  }
+  // f(first element) for the partial vectors, by two threads.
+  template <typename F>
+  __device__ __forceinline__ void edges(F&& f) const {
+    if (threadIdx.x == 0 && from == 1) f(first);
+    if (threadIdx.x == blockDim.x - 1 && to < n && (n > 1 || from == 0)) f(first + (n - 1) * VE);
+  }
+};
+
+// Which of a list's tokens may occur in it more than once: a token's bit (by
+// its low 13 bits) is set a second time.  Tokens that share a bit by chance
+// are marked too, which costs time, not results.
+struct Repeats {
+  static constexpr int kWords = 256;
+  uint32_t once[kWords], more[kWords];
+  __device__ __forceinline__ void clear() {
+    for (int i = threadIdx.x; i < kWords; i += blockDim.x) once[i] = more[i] = 0;
+  }
+  __device__ __forceinline__ void mark(int tok) {
+    const uint32_t word = (uint32_t)tok / 32 % kWords, bit = 1u << (tok & 31);
+    if (atomicOr(once + word, bit) & bit) atomicOr(more + word, bit);
+  }
+  __device__ __forceinline__ bool listed(int tok) const { return once[(uint32_t)tok / 32 % kWords] >> (tok & 31) & 1; }
+  __device__ __forceinline__ bool marked(int tok) const { return more[(uint32_t)tok / 32 % kWords] >> (tok & 31) & 1; }
+};
+
+// ---------------------------------------------------------------------------
 // Penalties, biases, masks.
 //
 //   x = l
@@ -29,177 +106,243 @@ constexpr int64_t kMaxVocab = (int64_t)1 << 30;  // element offsets inside a row
 //   x = x + bias            for the token's biases in list order
 //   not allowed:           x = -inf
 //
-// Every step is one IEEE fp32 operation.  A CTA takes one slice of one row: it
-// counts the history's tokens that fall into the slice in shared memory
-// (integer atomics: their order does not change the counts), marks the
-// slice's biased tokens, and then streams the slice.
+// Every step is one IEEE fp32 operation.  A CTA takes one slice of one row.
+// It counts the history's tokens that fall into the slice in shared memory
+// (integer atomics: their order does not change the counts) and then streams
+// the slice: a vector reads its eight counters in one or two 16-byte loads and
+// takes the slow way only if one is set; what the mask excludes is not read.
+// The few biased tokens are computed again and stored over, after a barrier.
 // ---------------------------------------------------------------------------
 
 constexpr int kProcThreads = 256;
-constexpr uint32_t kSeen = 0x80000000u;     // counter: the token occurs (prompt or not); low bits: its count
-constexpr uint32_t kNoBias = 0x7fffffffu;   // bias slot: no entry; else the first entry's position,
-constexpr uint32_t kRepeated = 0x80000000u; // with this bit when more entries name the token
+constexpr int kProcAhead = 4;  // vectors per thread in flight
 
 struct ProcArgs {
   const void* in;
   void* out;
   int64_t in_stride, out_stride;
   int vocab, split, vps;  // slices per row, vectors per slice
+  bool in_place;
   cnnue_logit_rules r;
   uint32_t* status;
 };
 
-template <typename TI, typename TO, bool HIST, bool BIAS>
-__global__ void __launch_bounds__(kProcThreads) process_kernel(const ProcArgs a) {
+// Counters of BITS bits per token: the high bit says that the token occurs,
+// the others how often after the prompt.  16 bits hold the counts of histories
+// of up to 32767 tokens.
+template <int BITS>
+struct Counters {
+  static constexpr uint32_t kSeen = 1u << (BITS - 1);
+  uint32_t* words;
+  __device__ __forceinline__ void clear(int tokens) {
+    for (int i = threadIdx.x; i < (tokens * BITS + 127) / 128; i += blockDim.x)  // the allocation is rounded up too
+      reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void see(int t, bool prompt) {
+    const int at = BITS == 16 ? 16 * (t & 1) : 0;
+    uint32_t* w = words + (BITS == 16 ? t >> 1 : t);
+    if (prompt)
+      atomicOr(w, kSeen << at);
+    else
+      atomicAdd(w, 1u << at);
+  }
+  __device__ __forceinline__ uint32_t of(int t) const {
+    return BITS == 16 ? words[t >> 1] >> 16 * (t & 1) & 0xffffu : words[t];
+  }
+  // Whether any of the N tokens from t on (a multiple of N) occurs.
+  template <int N>
+  __device__ __forceinline__ bool any(int t) const {
+    constexpr int kBytes = N * BITS / 8;
+    const char* p = (const char*)words + t * (BITS / 8);
+    uint32_t w = 0;
+    if (kBytes == 8) {
+      const uint2 a = *reinterpret_cast<const uint2*>(p);
+      w = a.x | a.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) {
+        const uint4 a = reinterpret_cast<const uint4*>(p)[i];
+        w |= a.x | a.y | a.z | a.w;
+      }
+    }
+    return w != 0;
+  }
+};
+
+struct Penalties {
+  float rep = 1.f, freq = 0.f, pres = 0.f;
+  // `c`: a counter without its high bit's place, 0 = the token does not occur.
+  template <int BITS>
+  __device__ __forceinline__ float apply(float x, uint32_t c) const {
+    if (c == 0) return x;
+    x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+    const uint32_t n = c & ~Counters<BITS>::kSeen;
+    return n ? __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)n)), pres) : x;
+  }
+};
+
+// HIST: 0, or the counters' bits.
+template <typename TI, typename TO, int HIST, bool BIAS>
+__global__ void __launch_bounds__(kProcThreads, 4) process_kernel(const __grid_constant__ ProcArgs a) {
   constexpr int VE = Vec<TI>::VE;
-  extern __shared__ uint32_t slots[];
+  constexpr int BITS = HIST ? HIST : 32;
+  extern __shared__ uint4 slots[];
+  __shared__ Repeats repeats;
   const int64_t row = blockIdx.x / a.split;
-  const int part = (int)(blockIdx.x % a.split);
+  const int part = (int)(blockIdx.x % a.split), stride = blockDim.x;
   const TI* in = (const TI*)a.in + row * a.in_stride;
   TO* out = (TO*)a.out + row * a.out_stride;
   const int shift = rows::shift_of(in);
-  const int v0 = part * a.vps;
-  const int lo = v0 * VE - shift;  // first token of the slice
-  const int width = a.vps * VE;    // tokens per slice
-  uint32_t* count = slots;
-  uint32_t* first = slots + (HIST ? width : 0);
+  const Slice<VE> slice(part, a.vps, shift, a.vocab);
+  const RowMask mask = row_mask(a.r, row, a.status, threadIdx.x == 0 && part == 0);
+  Counters<BITS> counters{reinterpret_cast<uint32_t*>(slots)};  // token t at t - slice.first
+  Penalties pen;
 
-  bool dead = false;  // the row's mask index is out of range: nothing is allowed
-  const uint32_t* mask = nullptr;
-  if (a.r.mask) {
-    const int64_t m = a.r.mask_index ? (int64_t)a.r.mask_index[row] : a.r.mask_rows == 1 ? 0 : row;
-    if (m >= a.r.mask_rows) {
-      dead = true;
-      if (threadIdx.x == 0 && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_INDEX);
-    } else if (m >= 0) {
-      mask = a.r.mask + m * a.r.mask_stride;
-    }
-  }
-
-  float rep = 1.f, freq = 0.f, pres = 0.f;
-  const int32_t* btok = nullptr;
-  const float* bval = nullptr;
-  if (HIST || BIAS) {
-    for (int i = threadIdx.x; i < width; i += kProcThreads) {
-      if (HIST) count[i] = 0;
-      if (BIAS) first[i] = kNoBias;
-    }
-    __syncthreads();
-  }
   if (HIST) {
-    if (a.r.repetition) rep = a.r.repetition[row];
-    if (a.r.frequency) freq = a.r.frequency[row];
-    if (a.r.presence) pres = a.r.presence[row];
+    counters.clear(slice.n * VE);
+    if (a.r.repetition) pen.rep = a.r.repetition[row];
+    if (a.r.frequency) pen.freq = a.r.frequency[row];
+    if (a.r.presence) pen.pres = a.r.presence[row];
     int64_t len = a.r.history_len;
     if (a.r.lengths) {
       const int64_t l = a.r.lengths[row];
-      if (l < 0 || l > len) {
-        if (threadIdx.x == 0 && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_OFFSETS);
-        len = l < 0 ? 0 : len;
-      } else {
-        len = l;
-      }
+      if ((l < 0 || l > len) && threadIdx.x == 0 && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_OFFSETS);
+      len = max((int64_t)0, min(l, len));
     }
     const int64_t prompt = a.r.prompt_lengths ? a.r.prompt_lengths[row] : 0;
     const bool wide = a.r.history_bytes == 8;
     const char* list = (const char*)a.r.history + row * a.r.history_stride * a.r.history_bytes;
-    for (int64_t i = threadIdx.x; i < len; i += kProcThreads) {
-      const int t = rows::token_at(list, i, wide);
-      if (t >= a.vocab) {
-        if (part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_INDEX);
-        continue;
+    bool bad = false;
+    __syncthreads();
+    for (int64_t i = threadIdx.x; i < len; i += 4 * stride) {
+      int t[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        t[j] = i + j * stride < len ? rows::token_at(list, i + j * stride, wide) : -1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        bad |= t[j] >= a.vocab;
+        if (t[j] >= slice.lo && t[j] < slice.hi) counters.see(t[j] - slice.first, i + j * stride < prompt);
       }
-      const int s = t - lo;
-      if (t < 0 || s < 0 || s >= width) continue;
-      if (i < prompt)
-        atomicOr(count + s, kSeen);
-      else
-        atomicAdd(count + s, 1u);
     }
+    if (bad && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_INDEX);
   }
+  const int32_t* btok = nullptr;
+  const float* bval = nullptr;
   if (BIAS) {
     btok = a.r.bias_tokens + row * a.r.bias_tokens_stride;
     bval = a.r.bias_values + row * a.r.bias_values_stride;
-    for (int64_t k = threadIdx.x; k < a.r.bias_count; k += kProcThreads) {
-      const int t = __ldg(btok + k);
-      if (t >= a.vocab) {
-        if (part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_INDEX);
-        continue;
-      }
-      const int s = t - lo;
-      if (t >= 0 && s >= 0 && s < width) atomicMin(first + s, (uint32_t)k);
-    }
+    repeats.clear();
     __syncthreads();
-    for (int64_t k = threadIdx.x; k < a.r.bias_count; k += kProcThreads) {
+    for (int64_t k = threadIdx.x; k < a.r.bias_count; k += stride) {
       const int t = __ldg(btok + k);
-      const int s = t - lo;
-      if (t < 0 || t >= a.vocab || s < 0 || s >= width) continue;
-      if ((first[s] & ~kRepeated) != (uint32_t)k) atomicOr(first + s, kRepeated);
+      if (t >= a.vocab && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_INDEX);
+      if (t >= slice.lo && t < slice.hi) repeats.mark(t);
     }
   }
   if (HIST || BIAS) __syncthreads();
 
-  const bool whole = rows::lines_up(out, shift);
-  const int v1 = v0 + a.vps;
-  for (int v = v0 + threadIdx.x; v < v1; v += kProcThreads) {
-    const int e0 = v * VE - shift;
-    const uint32_t inside = rows::inside<VE>(e0, a.vocab);
-    if (inside == 0) continue;
-    const uint32_t ok = dead ? 0 : mask ? rows::allowed<VE>(mask, e0, a.vocab) : inside;
-    float x[VE];
-    rows::load(in, e0, inside, ok, kNegInf, x);
-    if (HIST || BIAS) {
+  const bool lines_up = rows::lines_up(out, shift);
+  // the vector at e0 (the slice's vector i): penalties, mask, store
+  auto finish = [&](float* x, int i, int e0, uint32_t in_row, uint32_t ok, bool counted) {
+    if (HIST && counted) {
 #pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        if (!(ok >> i & 1)) continue;
-        if (HIST) {
-          const uint32_t c = count[e0 + i - lo];
-          if (c) {
-            x[i] = x[i] > 0.f ? __fdiv_rn(x[i], rep) : __fmul_rn(x[i], rep);
-            const uint32_t n = c & ~kSeen;
-            if (n) x[i] = __fsub_rn(__fsub_rn(x[i], __fmul_rn(freq, (float)n)), pres);
-          }
-        }
-        if (BIAS) {
-          const uint32_t f = first[e0 + i - lo];
-          if (f != kNoBias) {
-            if (!(f & kRepeated)) {
-              x[i] = __fadd_rn(x[i], __ldg(bval + f));
-            } else {  // rare: walk the list from the first entry on
-              for (int64_t k = f & ~kRepeated; k < a.r.bias_count; ++k)
-                if (__ldg(btok + k) == e0 + i) x[i] = __fadd_rn(x[i], __ldg(bval + k));
-            }
-          }
-        }
-      }
+      for (int j = 0; j < VE; ++j)
+        // in place, a biased token keeps its logit: the bias pass takes it from there
+        if ((ok >> j & 1) && !(BIAS && a.in_place && repeats.listed(e0 + j)))
+          x[j] = pen.apply<BITS>(x[j], counters.of(i * VE + j));
     }
-    rows::store<TO, VE>(out, e0, inside, whole, x);
+    if (ok != rows::kFull<VE>) {
+#pragma unroll
+      for (int j = 0; j < VE; ++j)
+        if (!(ok >> j & 1)) x[j] = kNegInf;
+    }
+    rows::store<TO, VE>(out, e0, in_row, lines_up, x);
+  };
+  slice.template each<kProcAhead>([&](int i, int e0, auto n) {
+    constexpr int N = decltype(n)::value;
+    uint4 raw[N];
+    uint32_t ok[N];
+    bool counted[N], skip[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int e = e0 + j * stride * VE;
+      ok[j] = mask.dead ? 0 : mask.words ? rows::allowed_whole<VE>(mask.words, e) : rows::kFull<VE>;
+      counted[j] = HIST && counters.template any<VE>((i + j * stride) * VE);
+      skip[j] = a.in_place && ok[j] == rows::kFull<VE> && !counted[j];  // nothing changes
+      raw[j] = make_uint4(0, 0, 0, 0);
+      if (ok[j] && !skip[j]) raw[j] = rows::load16(in + e);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (skip[j]) continue;
+      const int e = e0 + j * stride * VE;
+      float x[VE];
+      Vec<TI>::unpack(raw[j], x);
+      finish(x, i + j * stride, e, rows::kFull<VE>, ok[j], counted[j]);
+    }
+  });
+  slice.edges([&](int e0) {
+    const uint32_t in_row = rows::inside<VE>(e0, a.vocab);
+    const uint32_t ok = mask.dead ? 0 : mask.words ? rows::allowed<VE>(mask.words, e0, a.vocab) : in_row;
+    float x[VE];
+    Vec<TI>::unpack(rows::load_raw(in, e0, in_row, ok), x);
+    finish(x, (e0 - slice.first) / VE, e0, in_row, ok, true);
+  });
+
+  if (BIAS) {
+    __syncthreads();
+    for (int64_t k = threadIdx.x; k < a.r.bias_count; k += stride) {
+      const int t = __ldg(btok + k);
+      if (t < slice.lo || t >= slice.hi || !token_ok(mask, t)) continue;
+      float x = Vec<TI>::up(in[t]);
+      if (HIST) x = pen.apply<BITS>(x, counters.of(t - slice.first));
+      if (!repeats.marked(t)) {
+        x = __fadd_rn(x, __ldg(bval + k));
+      } else {  // in list order, by the thread of the token's first entry
+        bool earlier = false;
+        for (int64_t j = 0; j < a.r.bias_count; ++j) {
+          if (__ldg(btok + j) != t) continue;
+          earlier |= j < k;
+          x = __fadd_rn(x, __ldg(bval + j));
+        }
+        if (earlier) continue;
+      }
+      out[t] = Vec<TO>::down(x);
+    }
   }
 }
 
-template <typename TI, typename TO, bool HIST, bool BIAS>
-int launch_process(ProcArgs& a, int64_t n_rows, cudaStream_t s) {
+template <typename TI, typename TO, int HIST, bool BIAS>
+int launch_process(ProcArgs& a, int64_t n_rows, int64_t nv, cudaStream_t s) {
   constexpr int VE = Vec<TI>::VE;
-  const int64_t nv = rows::max_vectors<TI>(a.vocab);
-  // 8192 tokens per slice: 32 KB of counters and 32 KB of bias slots at most
-  const int64_t vps = std::min<int64_t>(nv, 8192 / VE);
+  // At most 32 KB of counters; the bits of Repeats stand for one token each.
+  const int64_t vps = std::min<int64_t>(nv, Repeats::kWords * 32 / VE);
   a.vps = (int)vps;
   a.split = (int)((nv + vps - 1) / vps);
-  const size_t smem = (size_t)vps * VE * 4 * ((HIST ? 1 : 0) + (BIAS ? 1 : 0));
+  const size_t smem = align_up((size_t)vps * VE * HIST / 8, 16);
+  const int threads = (int)std::min<int64_t>(kProcThreads, std::max<int64_t>(1, vps / (kProcAhead * 32)) * 32);
   if (n_rows * a.split > 0x7fffffff) return set_error(CNNUE_ERR_INVALID_ARG, "too many rows for one call");
-  if (smem > 48 * 1024)
-    CNNUE_CUDA_TRY(cudaFuncSetAttribute(process_kernel<TI, TO, HIST, BIAS>,
-                                        cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  process_kernel<TI, TO, HIST, BIAS><<<(unsigned)(n_rows * a.split), kProcThreads, smem, s>>>(a);
+  process_kernel<TI, TO, HIST, BIAS><<<(unsigned)(n_rows * a.split), threads, smem, s>>>(a);
   return check_launch_error("process_kernel");
+}
+
+// Vectors that cover a row: one more only where a row may start inside one.
+template <typename T>
+int64_t row_vectors(const void* p, int64_t stride, int64_t vocab) {
+  constexpr int VE = Vec<T>::VE;
+  return (uintptr_t)p % 16 == 0 && stride % VE == 0 ? (vocab + VE - 1) / VE : rows::max_vectors<T>(vocab);
 }
 
 template <typename TI, typename TO>
 int pick_process(ProcArgs& a, int64_t n_rows, cudaStream_t s) {
+  const int64_t nv = row_vectors<TI>(a.in, a.in_stride, a.vocab);
   const bool hist = a.r.history && a.r.history_len > 0 && (a.r.repetition || a.r.frequency || a.r.presence);
   const bool bias = a.r.bias_tokens && a.r.bias_count > 0;
-  if (hist) return bias ? launch_process<TI, TO, true, true>(a, n_rows, s) : launch_process<TI, TO, true, false>(a, n_rows, s);
-  return bias ? launch_process<TI, TO, false, true>(a, n_rows, s) : launch_process<TI, TO, false, false>(a, n_rows, s);
+  if (!hist) return bias ? launch_process<TI, TO, 0, true>(a, n_rows, nv, s) : launch_process<TI, TO, 0, false>(a, n_rows, nv, s);
+  if (a.r.history_len < 32768)
+    return bias ? launch_process<TI, TO, 16, true>(a, n_rows, nv, s) : launch_process<TI, TO, 16, false>(a, n_rows, nv, s);
+  return bias ? launch_process<TI, TO, 32, true>(a, n_rows, nv, s) : launch_process<TI, TO, 32, false>(a, n_rows, nv, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -227,26 +370,6 @@ struct LossArgs {
   int64_t grad_stride;
   uint32_t* status;
 };
-
-struct RowMask {
-  const uint32_t* words;  // null: everything is allowed (unless dead)
-  bool dead;
-};
-__device__ __forceinline__ RowMask row_mask(const cnnue_loss_targets& t, int64_t row, uint32_t* status, bool tell) {
-  RowMask m{nullptr, false};
-  if (!t.mask) return m;
-  const int64_t i = t.mask_index ? (int64_t)t.mask_index[row] : t.mask_rows == 1 ? 0 : row;
-  if (i >= t.mask_rows) {
-    m.dead = true;
-    if (tell) atomicOr(status, CNNUE_STATUS_BAD_INDEX);
-  } else if (i >= 0) {
-    m.words = t.mask + i * t.mask_stride;
-  }
-  return m;
-}
-__device__ __forceinline__ bool token_ok(const RowMask& m, int t) {
-  return !m.dead && (!m.words || (__ldg(m.words + (t >> 5)) >> (t & 31) & 1));
-}
 
 // Exponentials are exp2(x c - B) with c = log2(e) in fp32 and B = m c rounded:
 // one fused operation per element before the instruction, and because every
@@ -345,22 +468,6 @@ __device__ __forceinline__ Sums join_all(Sums v, bool targets, Sums* shared, int
 __device__ __forceinline__ void cluster_done(int ctas) {
   if (ctas > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
-
-// Which of a list's tokens may occur in it more than once: a token's bit (by
-// its low 13 bits) is set a second time.  Tokens that share a bit by chance
-// are marked too, which costs time, not results.
-struct Repeats {
-  static constexpr int kWords = 256;
-  uint32_t once[kWords], more[kWords];
-  __device__ __forceinline__ void clear() {
-    for (int i = threadIdx.x; i < kWords; i += blockDim.x) once[i] = more[i] = 0;
-  }
-  __device__ __forceinline__ void mark(int tok) {
-    const uint32_t word = (uint32_t)tok / 32 % kWords, bit = 1u << (tok & 31);
-    if (atomicOr(once + word, bit) & bit) atomicOr(more + word, bit);
-  }
-  __device__ __forceinline__ bool marked(int tok) const { return more[(uint32_t)tok / 32 % kWords] >> (tok & 31) & 1; }
-};
 
 // One row's tensors as a CTA sees them.
 template <typename T>
@@ -536,40 +643,6 @@ __device__ __forceinline__ void LossRow<T>::edge_grad(int e0, bool none, T* g, f
   grad_vector<T, DENSE>(*this, raw, e0, ok, false, m, c, w, x);
   rows::store<T, VE>(g, e0, in, false, x);
 }
-
-// A CTA's slice of a row: vectors 0 .. n - 1, vector i at element first + i VE.
-// All but the row's first and last are whole; whole ones are [from, to).
-template <int VE>
-struct Slice {
-  int first, n, from, to, lo, hi;
-  __device__ __forceinline__ Slice(int rank, int vps, int shift, int vocab) {
-    first = rank * vps * VE - shift;
-    n = max(0, min(vps, (shift + vocab + VE - 1) / VE - rank * vps));
-    from = n > 0 && first < 0 ? 1 : 0;
-    to = n > 0 && first + n * VE > vocab ? n - 1 : n;
-    lo = max(0, first);
-    hi = min(vocab, first + n * VE);
-  }
-  // f(i, e0, n) for this thread's share of the whole vectors, n = N (the
-  // vectors i + j blockDim, at e0 + j blockDim VE) and 1 for what is left.  The
-  // same share at every call.
-  template <int N, typename F>
-  __device__ __forceinline__ void each(F&& f) const {
-    const int stride = blockDim.x;
-    int i = from + threadIdx.x;
-    for (; i + (N - 1) * stride < to; i += N * stride) f(i, first + i * VE, std::integral_constant<int, N>{});
-    if (N > 1) {
-#pragma unroll 1
-      for (; i < to; i += stride) f(i, first + i * VE, std::integral_constant<int, 1>{});
-    }
-  }
-  // f(first element) for the partial vectors, by two threads.
-  template <typename F>
-  __device__ __forceinline__ void edges(F&& f) const {
-    if (threadIdx.x == 0 && from == 1) f(first);
-    if (threadIdx.x == blockDim.x - 1 && to < n && (n > 1 || from == 0)) f(first + (n - 1) * VE);
-  }
-};
 
 constexpr int kTogether = 4;  // vectors per thread in the gradient loop
 constexpr int kAhead = 4;     // vectors per thread between two looks at the running maximum
@@ -821,13 +894,6 @@ int launch_loss(const LossArgs& a, int threads, cudaStream_t s) {
   return check_launch_error("loss_kernel");
 }
 
-// Vectors that cover a row: one more only where a row may start inside one.
-template <typename T>
-int64_t row_vectors(const void* p, int64_t stride, int64_t vocab) {
-  constexpr int VE = Vec<T>::VE;
-  return (uintptr_t)p % 16 == 0 && stride % VE == 0 ? (vocab + VE - 1) / VE : rows::max_vectors<T>(vocab);
-}
-
 // A slice is at most 64 KB of shared memory, 3 CTAs per SM.  Measured at 1024 x
 // 131072 bf16: 117 us with 4 CTAs of 64 KB per row, 139 with 8 of 32 KB (twice
 // the threads' fixed work, and more to wait for in each cluster).
@@ -953,17 +1019,17 @@ int cnnue_logits_process(const void* d_logits, int64_t logits_stride, int logits
   const cnnue_logit_rules& r = *rules;
   if (r.history) {
     if (r.history_bytes != 4 && r.history_bytes != 8) return set_error(CNNUE_ERR_INVALID_ARG, "history_bytes");
-    if (r.history_len < 0 || r.history_len >= kSeen || r.history_stride < 0)
+    if (r.history_len < 0 || r.history_len > 0x7fffffff || r.history_stride < 0)
       return set_error(CNNUE_ERR_INVALID_ARG, "history: length or stride");
   } else if (r.repetition || r.frequency || r.presence || r.lengths || r.prompt_lengths) {
     return set_error(CNNUE_ERR_INVALID_ARG, "penalties without a history");
   }
   if ((r.bias_tokens != nullptr) != (r.bias_values != nullptr))
     return set_error(CNNUE_ERR_INVALID_ARG, "bias tokens and values come together");
-  if (r.bias_count < 0 || r.bias_count >= kNoBias || r.bias_tokens_stride < 0 || r.bias_values_stride < 0)
+  if (r.bias_count < 0 || r.bias_count > 0x7fffffff || r.bias_tokens_stride < 0 || r.bias_values_stride < 0)
     return set_error(CNNUE_ERR_INVALID_ARG, "bias: count or stride");
   if (int st = check_mask(r.mask, r.mask_stride, r.mask_rows, r.mask_index, n_rows, vocab)) return st;
-  ProcArgs a{d_logits, d_out, logits_stride, out_stride, (int)vocab, 0, 0, r, d_status};
+  ProcArgs a{d_logits, d_out, logits_stride, out_stride, (int)vocab, 0, 0, in_place, r, d_status};
   cudaStream_t s = (cudaStream_t)stream;
   if (logits_type == CNNUE_F32) return pick_process<float, float>(a, n_rows, s);
   if (logits_type == CNNUE_BF16)

@@ -16,12 +16,13 @@ stream, allocate only their results and can be captured in a CUDA graph when
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import numpy as np
 import torch
 
-from ._lib import LogitRules, LossTargets, check, lib
+from ._lib import check, lib
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -40,6 +41,14 @@ def pack_mask(allowed) -> "torch.Tensor | np.ndarray":
     return torch.where(w >= 1 << 31, w - (1 << 32), w).to(torch.int32)
 
 
+# The C structs as bytes (native layout): much quicker to fill than field by
+# field, and these calls run once per generated token.
+_RULES = struct.Struct("@PqqiPPPPPPqPqqPqqP")    # cnnue_logit_rules
+_TARGETS = struct.Struct("@PqiPqiPqqPqqPP")       # cnnue_loss_targets
+_NO_MASK = (0, 0, 0, 0)
+_INTS = {torch.int32: 4, torch.int64: 8}
+
+
 def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
     if x.dim() != 2:
         raise ValueError(f"{name} must be [rows, vocab], got {tuple(x.shape)}")
@@ -47,90 +56,93 @@ def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
         raise ValueError(f"{name} must be a CUDA tensor")
     if x.dtype not in _TYPES:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
-    return x if x.shape[1] <= 1 or x.stride(1) == 1 else x.contiguous()
+    return x if x.stride(1) == 1 or x.size(1) <= 1 else x.contiguous()
 
 
-def _per_row(x: Optional[torch.Tensor], like: torch.Tensor, dtype: torch.dtype, name: str, keep: list):
-    """Pointer of a per-row vector, or None."""
+def _per_row(x: Optional[torch.Tensor], n: int, dev: int, dtype: torch.dtype, name: str, keep: list) -> int:
+    """Address of a per-row vector, 0 for None."""
     if x is None:
-        return None
-    if x.device != like.device:
-        raise ValueError(f"{name} must be on {like.device}, is on {x.device}")
-    if x.dtype != dtype:
+        return 0
+    if x.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {x.dtype}")
-    if x.shape != like.shape[:1]:
-        raise ValueError(f"{name} must be [{like.shape[0]}], got {tuple(x.shape)}")
+    if x.get_device() != dev:
+        raise ValueError(f"{name} must be on cuda:{dev}, is on {x.device}")
+    if x.dim() != 1 or x.size(0) != n:
+        raise ValueError(f"{name} must be [{n}], got {tuple(x.shape)}")
     if not x.is_contiguous():
         x = x.contiguous()
         keep.append(x)
     return x.data_ptr()
 
 
-def _lists(x: torch.Tensor, like: torch.Tensor, dtypes, name: str, keep: list) -> Tuple[int, int, int]:
-    """(pointer, row stride, length) of lists [rows, n], or [n] for all rows."""
-    if x.device != like.device:
-        raise ValueError(f"{name} must be on {like.device}, is on {x.device}")
+def _lists(x: torch.Tensor, n: int, dev: int, dtypes, name: str, keep: list) -> Tuple[int, int, int]:
+    """(address, row stride, length) of lists [rows, n], or [n] for all rows."""
     if x.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {x.dtype}")
-    if x.dim() not in (1, 2) or (x.dim() == 2 and x.shape[0] != like.shape[0]):
-        raise ValueError(f"{name} must be [{like.shape[0]}, n] or [n], got {tuple(x.shape)}")
-    n = x.shape[-1]
-    if n > 1 and x.stride(-1) != 1:
+    if x.get_device() != dev:
+        raise ValueError(f"{name} must be on cuda:{dev}, is on {x.device}")
+    dim = x.dim()
+    if dim not in (1, 2) or (dim == 2 and x.size(0) != n):
+        raise ValueError(f"{name} must be [{n}, n] or [n], got {tuple(x.shape)}")
+    length = x.size(-1)
+    if length > 1 and x.stride(-1) != 1:
         x = x.contiguous()
         keep.append(x)
     # an empty list has no storage and is never read: any address says that it is there
-    return x.data_ptr() or like.data_ptr(), (x.stride(0) if x.dim() == 2 else 0), n
+    return x.data_ptr() or 1 << 12, (x.stride(0) if dim == 2 else 0), length
 
 
-def _set_mask(s, mask, mask_index, like: torch.Tensor, keep: list) -> None:
-    """Fills the mask fields of a LogitRules or LossTargets."""
+def _mask(mask: Optional[torch.Tensor], mask_index, n: int, vocab: int, dev: int, keep: list):
+    """The mask fields of a struct: address, stride, rows, index."""
     if mask is None:
         if mask_index is not None:
             raise ValueError("mask_index without a mask")
-        return
-    if mask.device != like.device:
-        raise ValueError(f"mask must be on {like.device}, is on {mask.device}")
-    if mask.dtype != torch.int32:
+        return _NO_MASK
+    if mask.dtype is not torch.int32:
         raise TypeError(f"mask must hold packed int32 words (pack_mask), got {mask.dtype}")
-    words = (like.shape[1] + 31) // 32
-    if mask.dim() not in (1, 2) or mask.shape[-1] != words:
+    if mask.get_device() != dev:
+        raise ValueError(f"mask must be on cuda:{dev}, is on {mask.device}")
+    words, dim = (vocab + 31) // 32, mask.dim()
+    if dim not in (1, 2) or mask.size(-1) != words:
         raise ValueError(f"mask must be [masks, {words}] or [{words}], got {tuple(mask.shape)}")
     if words > 1 and mask.stride(-1) != 1:
         mask = mask.contiguous()
         keep.append(mask)
-    n = 1 if mask.dim() == 1 else mask.shape[0]
-    if mask_index is None and n != 1 and n != like.shape[0]:
-        raise ValueError(f"mask has {n} rows for {like.shape[0]} rows of logits and no mask_index")
-    s.mask, s.mask_stride, s.mask_rows = mask.data_ptr(), (0 if mask.dim() == 1 else mask.stride(0)), n
-    s.mask_index = _per_row(mask_index, like, torch.int32, "mask_index", keep)
+    m = 1 if dim == 1 else mask.size(0)
+    if mask_index is None and m != 1 and m != n:
+        raise ValueError(f"mask has {m} rows for {n} rows of logits and no mask_index")
+    return mask.data_ptr() or 1 << 12, (0 if dim == 1 else mask.stride(0)), m, \
+        _per_row(mask_index, n, dev, torch.int32, "mask_index", keep)
 
 
-class _Call:
-    """The status word, the stream and the device of one call: with `status`
-    None the word is read here (a host synchronisation) and raised."""
+def _current_stream(dev: int) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
 
-    def __init__(self, like: torch.Tensor, status: Optional[torch.Tensor]):
-        self.device = like.device
-        self.own = status is None
-        if self.own:
-            status = torch.zeros(1, dtype=torch.int32, device=like.device)
-        elif status.device != like.device or status.dtype != torch.int32 or status.numel() < 1:
-            raise ValueError(f"status must be an int32 tensor on {like.device}")
-        self.status = status
 
-    def __call__(self, name: str, *args) -> None:
-        if torch.cuda.current_device() != self.device.index:
-            with torch.cuda.device(self.device):
-                return self._run(name, *args)
-        return self._run(name, *args)
+# the same handle without the Stream object around it, where torch has the call
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
 
-    def _run(self, name: str, *args) -> None:
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        check(getattr(lib(), name)(*args, self.status.data_ptr(), stream), name)
-        if self.own:
-            st = C.c_int(0)
-            check(lib().cnnue_read_status(self.status.data_ptr(), stream, C.byref(st)), "cnnue_read_status")
-            check(st.value, f"{name} (kernel status)")
+
+def _call(name: str, dev: int, status: Optional[torch.Tensor], *args) -> None:
+    """One entry point on the device's current stream.  With `status` None the
+    kernels' status word is read here (a host synchronisation) and raised."""
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return _call(name, dev, status, *args)
+    own = status is None
+    if own:
+        status = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", dev))
+    elif status.dtype is not torch.int32 or status.get_device() != dev or status.numel() < 1:
+        raise ValueError(f"status must be an int32 tensor on cuda:{dev}")
+    stream = _stream(dev)
+    handle = lib()
+    st = getattr(handle, name)(*args, status.data_ptr(), stream)
+    if st:
+        check(st, name)
+    if own:
+        word = C.c_int(0)
+        check(handle.cnnue_read_status(status.data_ptr(), stream, C.byref(word)), "cnnue_read_status")
+        check(word.value, f"{name} (kernel status)")
 
 
 def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None,
@@ -165,79 +177,97 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     if torch.is_grad_enabled() and logits.requires_grad:
         raise ValueError("process_logits is not differentiable: detach the logits or use policy_loss")
     z = _rows(logits, "logits")
+    n, vocab = z.shape
+    dev = z.get_device()
+    code = _TYPES[z.dtype]
     if out is None:
-        dtype = z.dtype if out_dtype is None else out_dtype
-        if dtype != z.dtype and dtype != torch.float32:
-            raise TypeError(f"out_dtype must be {z.dtype} or float32, got {dtype}")
-        out = torch.empty(z.shape, dtype=dtype, device=z.device)
+        if out_dtype is None or out_dtype is z.dtype:
+            out, out_code = torch.empty_like(z), code
+        elif out_dtype is torch.float32:
+            out, out_code = torch.empty_like(z, dtype=torch.float32), 0
+        else:
+            raise TypeError(f"out_dtype must be {z.dtype} or float32, got {out_dtype}")
     else:
-        if out.shape != z.shape or out.device != z.device:
+        if out.shape != z.shape or out.get_device() != dev:
             raise ValueError(f"out must be {tuple(z.shape)} on {z.device}, is {tuple(out.shape)} on {out.device}")
         if (out.dtype != z.dtype and out.dtype != torch.float32) or (out_dtype is not None and out.dtype != out_dtype):
             raise TypeError(f"out must be {z.dtype} or float32 (and out_dtype, if given), got {out.dtype}")
-        if out.shape[1] > 1 and out.stride(1) != 1:
+        if vocab > 1 and out.stride(1) != 1:
             raise ValueError("out: the vocabulary must be contiguous")
         if torch.is_grad_enabled() and out.requires_grad:
             raise ValueError("out requires a gradient")
-    keep: list = [z]
-    r = LogitRules()
+        out_code = _TYPES[out.dtype]
+    keep: list = []
     if history is not None:
-        r.history, r.history_stride, r.history_len = _lists(history, z, (torch.int32, torch.int64), "history", keep)
-        r.history_bytes = history.element_size()
-        r.lengths = _per_row(lengths, z, torch.int32, "lengths", keep)
-        r.prompt_lengths = _per_row(prompt_lengths, z, torch.int32, "prompt_lengths", keep)
-        r.repetition = _per_row(repetition, z, torch.float32, "repetition", keep)
-        r.frequency = _per_row(frequency, z, torch.float32, "frequency", keep)
-        r.presence = _per_row(presence, z, torch.float32, "presence", keep)
-    elif any(x is not None for x in (lengths, prompt_lengths, repetition, frequency, presence)):
-        raise ValueError("penalties need a history")
-    if (bias_tokens is None) != (bias_values is None):
-        raise ValueError("bias_tokens and bias_values come together")
-    if bias_tokens is not None:
+        f32 = torch.float32
+        h, h_stride, h_len = _lists(history, n, dev, _INTS, "history", keep)
+        part = (h, h_stride, h_len, _INTS[history.dtype], _per_row(lengths, n, dev, torch.int32, "lengths", keep),
+                _per_row(prompt_lengths, n, dev, torch.int32, "prompt_lengths", keep),
+                _per_row(repetition, n, dev, f32, "repetition", keep), _per_row(frequency, n, dev, f32, "frequency", keep),
+                _per_row(presence, n, dev, f32, "presence", keep))
+    else:
+        for x in (lengths, prompt_lengths, repetition, frequency, presence):
+            if x is not None:
+                raise ValueError("penalties need a history")
+        part = (0, 0, 0, 0, 0, 0, 0, 0, 0)
+    if bias_tokens is not None and bias_values is not None:
         if bias_tokens.shape != bias_values.shape:
             raise ValueError(f"bias_tokens {tuple(bias_tokens.shape)} and bias_values {tuple(bias_values.shape)} differ")
-        r.bias_tokens, r.bias_tokens_stride, r.bias_count = _lists(bias_tokens, z, (torch.int32,), "bias_tokens", keep)
-        r.bias_values, r.bias_values_stride, _ = _lists(bias_values, z, (torch.float32,), "bias_values", keep)
-    _set_mask(r, mask, mask_index, z, keep)
-    _Call(z, status)("cnnue_logits_process", z.data_ptr(), z.stride(0), _TYPES[z.dtype], out.data_ptr(), out.stride(0),
-                     _TYPES[out.dtype], z.shape[0], z.shape[1], C.addressof(r))
+        t, t_stride, count = _lists(bias_tokens, n, dev, (torch.int32,), "bias_tokens", keep)
+        v, v_stride, _ = _lists(bias_values, n, dev, (torch.float32,), "bias_values", keep)
+        bias = (t, t_stride, v, v_stride, count)
+    elif bias_tokens is None and bias_values is None:
+        bias = (0, 0, 0, 0, 0)
+    else:
+        raise ValueError("bias_tokens and bias_values come together")
+    rules = _RULES.pack(*part, *bias, *_mask(mask, mask_index, n, vocab, dev, keep))
+    _call("cnnue_logits_process", dev, status, z.data_ptr(), z.stride(0), code, out.data_ptr(), out.stride(0), out_code, n,
+          vocab, rules)
     return out
 
 
-def _targets(z: torch.Tensor, targets, target_index, target_prob, mask, mask_index, weights, keep: list) -> LossTargets:
-    t = LossTargets()
-    if (targets is None) == (target_index is None):
-        raise ValueError("give either dense targets or target_index")
+def _targets(z: torch.Tensor, targets, target_index, target_prob, mask, mask_index, weights, keep: list) -> bytes:
+    n, vocab = z.shape
+    dev = z.get_device()
     if targets is not None:
+        if target_index is not None:
+            raise ValueError("give either dense targets or target_index")
         if target_prob is not None:
             raise ValueError("target_prob goes with target_index")
-        if targets.shape != z.shape or targets.device != z.device:
+        if targets.shape != z.shape or targets.get_device() != dev:
             raise ValueError(f"targets must be {tuple(z.shape)} on {z.device}, are {tuple(targets.shape)} on {targets.device}")
         d = _rows(targets, "targets")
-        keep.append(d)
-        t.dense, t.dense_stride, t.dense_type = d.data_ptr(), d.stride(0), _TYPES[d.dtype]
+        if d is not targets:
+            keep.append(d)
+        part = (d.data_ptr(), d.stride(0), _TYPES[d.dtype], 0, 0, 0, 0, 0, 0)
     else:
+        if target_index is None:
+            raise ValueError("give either dense targets or target_index")
         if target_index.dim() == 1:  # labels: one token per row
             target_index = target_index[:, None]
             if target_prob is not None and target_prob.dim() == 1:
                 target_prob = target_prob[:, None]
         if target_index.dim() != 2:
             raise ValueError(f"target_index must be [rows] or [rows, n], got {tuple(target_index.shape)}")
-        t.index, t.index_stride, t.count = _lists(target_index, z, (torch.int32, torch.int64), "target_index", keep)
-        t.index_bytes = target_index.element_size()
+        i, i_stride, count = _lists(target_index, n, dev, _INTS, "target_index", keep)
+        p = p_stride = 0
         if target_prob is not None:
             if target_prob.shape != target_index.shape:
                 raise ValueError(f"target_prob must be {tuple(target_index.shape)}, got {tuple(target_prob.shape)}")
-            t.prob, t.prob_stride, _ = _lists(target_prob, z, (torch.float32,), "target_prob", keep)
-    _set_mask(t, mask, mask_index, z, keep)
-    t.weights = _per_row(weights, z, torch.float32, "weights", keep)
-    return t
+            p, p_stride, _ = _lists(target_prob, n, dev, (torch.float32,), "target_prob", keep)
+        part = (0, 0, 0, i, i_stride, _INTS[target_index.dtype], p, p_stride, count)
+    return _TARGETS.pack(*part, *_mask(mask, mask_index, n, vocab, dev, keep),
+                         _per_row(weights, n, dev, torch.float32, "weights", keep))
 
 
-def _refuse_gradients(**named) -> None:
-    for name, x in named.items():
+def _refuse_gradients(*tensors) -> None:
+    for x in tensors:
         if x is not None and x.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{name}: the loss is differentiable in the logits only")
+            raise ValueError("targets, target_prob and weights: the loss is differentiable in the logits only")
+
+
+def _addresses(tensors) -> list:
+    return [0 if x is None else x.data_ptr() for x in tensors]
 
 
 class _PolicyLoss(torch.autograd.Function):
@@ -246,25 +276,36 @@ class _PolicyLoss(torch.autograd.Function):
         z = _rows(logits, "logits")
         keep: list = []
         t = _targets(z, targets, target_index, target_prob, mask, mask_index, weights, keep)
-        loss = torch.empty(z.shape[0], dtype=torch.float32, device=z.device)
-        stats = torch.empty((z.shape[0], 3), dtype=torch.float32, device=z.device)
-        _Call(z, status)("cnnue_policy_loss_fwd", z.data_ptr(), z.stride(0), _TYPES[z.dtype], z.shape[0], z.shape[1],
-                         C.addressof(t), loss.data_ptr(), stats.data_ptr())
-        ctx.save_for_backward(logits, targets, target_index, target_prob, mask, mask_index, weights, stats)
+        n, vocab = z.shape
+        dev = z.get_device()
+        loss = z.new_empty(n, dtype=torch.float32)
+        stats = z.new_empty(3 * n, dtype=torch.float32)
+        _call("cnnue_policy_loss_fwd", dev, status, z.data_ptr(), z.stride(0), _TYPES[z.dtype], n, vocab, t,
+              loss.data_ptr(), stats.data_ptr())
+        saved = (logits, targets, target_index, target_prob, mask, mask_index, weights, stats)
+        ctx.save_for_backward(*saved)
         ctx.status = status
+        # for a backward pass over the same storage (saved-tensor hooks may bring another): the struct, and what it
+        # points to that is a copy (the rest is held by the saved tensors alone, and freed with them)
+        ctx.packed = (_addresses(saved), None if z is logits else z, t, keep)
         return loss
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, upstream):
-        logits, targets, target_index, target_prob, mask, mask_index, weights, stats = ctx.saved_tensors
-        z = _rows(logits, "logits")
-        keep: list = []
-        t = _targets(z, targets, target_index, target_prob, mask, mask_index, weights, keep)
-        up = upstream.float().contiguous()
-        grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        _Call(z, ctx.status)("cnnue_policy_loss_bwd", z.data_ptr(), z.stride(0), _TYPES[z.dtype], z.shape[0],
-                             z.shape[1], C.addressof(t), stats.data_ptr(), up.data_ptr(), grad.data_ptr(),
-                             grad.stride(0))
+        saved = ctx.saved_tensors
+        stats = saved[7]
+        addresses, z, t, keep = ctx.packed
+        if _addresses(saved) != addresses:
+            z, keep = _rows(saved[0], "logits"), []
+            t = _targets(z, *saved[1:7], keep)
+        elif z is None:
+            z = saved[0]
+        n, vocab = z.shape
+        up = upstream if upstream.dtype is torch.float32 and upstream.is_contiguous() else upstream.float().contiguous()
+        grad = torch.empty_like(z)
+        _call("cnnue_policy_loss_bwd", z.get_device(), ctx.status, z.data_ptr(), z.stride(0), _TYPES[z.dtype], n, vocab, t,
+              stats.data_ptr(), up.data_ptr(), grad.data_ptr(), grad.stride(0))
         return grad, None, None, None, None, None, None, None
 
 
@@ -285,7 +326,7 @@ def policy_loss(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, *,
     mean.  A row with nothing allowed, or of weight 0, has loss 0 and gradient
     0; a NaN at an allowed token makes its row NaN.  A listed token >= V raises
     CnnueError, or sets a bit of `status` (int32 device tensor) when given."""
-    _refuse_gradients(targets=targets, target_prob=target_prob, weights=weights)
+    _refuse_gradients(targets, target_prob, weights)
     return _PolicyLoss.apply(logits, targets, target_index, target_prob, mask, mask_index, weights, status)
 
 
@@ -298,18 +339,22 @@ def policy_loss_grad(logits: torch.Tensor, targets: Optional[torch.Tensor] = Non
     logits' dtype), in one pass over the logits: policy_loss and its backward
     for training loops that know the row weights beforehand.  Arguments as in
     policy_loss; `grad`: where to write the gradient (not the logits)."""
-    _refuse_gradients(targets=targets, target_prob=target_prob, weights=weights)
-    z = _rows(logits.detach(), "logits")
+    _refuse_gradients(targets, target_prob, weights)
+    z = _rows(logits, "logits")
     keep: list = []
     t = _targets(z, targets, target_index, target_prob, mask, mask_index, weights, keep)
+    n, vocab = z.shape
+    dev = z.get_device()
     if grad is None:
-        grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        grad = torch.empty_like(z)
     else:
-        if grad.shape != z.shape or grad.device != z.device or grad.dtype != z.dtype:
+        if grad.shape != z.shape or grad.get_device() != dev or grad.dtype != z.dtype:
             raise ValueError(f"grad must be {z.dtype} {tuple(z.shape)} on {z.device}")
-        if grad.shape[1] > 1 and grad.stride(1) != 1:
+        if vocab > 1 and grad.stride(1) != 1:
             raise ValueError("grad: the vocabulary must be contiguous")
-    loss = torch.empty(z.shape[0], dtype=torch.float32, device=z.device)
-    _Call(z, status)("cnnue_policy_loss_grad", z.data_ptr(), z.stride(0), _TYPES[z.dtype], z.shape[0], z.shape[1],
-                     C.addressof(t), loss.data_ptr(), grad.data_ptr(), grad.stride(0))
+        if torch.is_grad_enabled() and grad.requires_grad:
+            raise ValueError("grad requires a gradient")
+    loss = z.new_empty(n, dtype=torch.float32)
+    _call("cnnue_policy_loss_grad", dev, status, z.data_ptr(), z.stride(0), _TYPES[z.dtype], n, vocab, t, loss.data_ptr(),
+          grad.data_ptr(), grad.stride(0))
     return loss, grad

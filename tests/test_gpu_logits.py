@@ -112,6 +112,26 @@ def test_process_strides_in_place_and_neighbours(pad, offset, dtype):
     assert torch.equal(buf, before), "in place: wrote outside the rows"
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [100, 2086, 20_001])
+def test_process_in_place_with_penalties_biases_and_masks_rounds_once(vocab, dtype):
+    """The same bits as out of place: biased tokens among the penalised ones, repeated, masked."""
+    g = gen(vocab)
+    R = 4
+    x = rows(R, vocab, dtype, g)
+    h = history_of(R, vocab, 200, g)
+    kw = dict(history=h, repetition=1 + torch.rand(R, generator=g), frequency=torch.rand(R, generator=g),
+              bias_tokens=torch.cat([h[:, :20], h[:, 5:10], torch.randint(0, vocab, (R, 10), generator=g).int()], 1),
+              bias_values=torch.randn(R, 35, generator=g), mask=mask_of(R, vocab, 0.8, g))
+    d = {k: dev(t) for k, t in kw.items()}
+    out = lg.process_logits(dev(x), **d)
+    want, bound = ref.process(x, **kw)
+    ref.close(out, want, bound, dtype)
+    y = dev(x).clone()
+    lg.process_logits(y, out=y, **d)
+    assert torch.equal(y, out)
+
+
 def test_process_broadcast_row_and_transposed_logits():
     g = gen(5)
     x = rows(1, 500, torch.float32, g)

@@ -65,6 +65,15 @@ def rules(**kw):
     return C.addressof(r), r
 
 
+@pytest.mark.parametrize("packed,declared", [(logits._RULES, _lib.LogitRules), (logits._TARGETS, _lib.LossTargets)])
+def test_packed_structs_have_the_declared_layout(packed, declared):
+    values = list(range(1, len(declared._fields_) + 1))
+    data = packed.pack(*values)
+    assert len(data) == C.sizeof(declared)
+    back = declared.from_buffer_copy(data)
+    assert [getattr(back, name) for name, _ in declared._fields_] == values
+
+
 A, B, S = 1 << 20, 1 << 24, 1 << 28  # addresses that no call below gets to use
 
 
