@@ -108,10 +108,13 @@ struct Repeats {
 //
 // Every step is one IEEE fp32 operation.  A CTA takes one slice of one row.
 // It counts the history's tokens that fall into the slice in shared memory
-// (integer atomics: their order does not change the counts) and then streams
-// the slice: a vector reads its eight counters in one or two 16-byte loads and
-// takes the slow way only if one is set; what the mask excludes is not read.
-// The few biased tokens are computed again and stored over, after a barrier.
+// (integer atomics: their order does not change the counts) and notes each
+// token's first occurrence in a list; it streams the slice through the mask
+// (what that excludes is not read); and after a barrier it computes the listed
+// tokens, whose logits are in L2 by then, and the biased ones, and stores them
+// over.  With the counters looked up for every vector on its way instead, most
+// warps held some penalised token and went the slow way: 253 us for 2048 x
+// 50001 fp16 with 512 tokens of history.
 // ---------------------------------------------------------------------------
 
 constexpr int kProcThreads = 256;
@@ -129,43 +132,27 @@ struct ProcArgs {
 
 // Counters of BITS bits per token: the high bit says that the token occurs,
 // the others how often after the prompt.  16 bits hold the counts of histories
-// of up to 32767 tokens.
+// of up to 32767 tokens.  Then the list of the tokens that occur, in no order.
 template <int BITS>
 struct Counters {
   static constexpr uint32_t kSeen = 1u << (BITS - 1);
   uint32_t* words;
-  __device__ __forceinline__ void clear(int tokens) {
-    for (int i = threadIdx.x; i < (tokens * BITS + 127) / 128; i += blockDim.x)  // the allocation is rounded up too
+  uint16_t* list;
+  int* listed;
+  static __host__ __device__ int64_t count_bytes(int64_t tokens) { return (tokens * BITS / 8 + 15) / 16 * 16; }
+  __device__ __forceinline__ void clear(int tokens) const {
+    for (int i = threadIdx.x; i < count_bytes(tokens) / 16; i += blockDim.x)
       reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x == 0) *listed = 0;
   }
-  __device__ __forceinline__ void see(int t, bool prompt) {
+  __device__ __forceinline__ void see(int t, bool prompt) const {
     const int at = BITS == 16 ? 16 * (t & 1) : 0;
     uint32_t* w = words + (BITS == 16 ? t >> 1 : t);
-    if (prompt)
-      atomicOr(w, kSeen << at);
-    else
-      atomicAdd(w, 1u << at);
+    const uint32_t before = prompt ? atomicOr(w, kSeen << at) : atomicAdd(w, 1u << at);
+    if ((BITS == 16 ? before >> at & 0xffffu : before) == 0) list[atomicAdd(listed, 1)] = (uint16_t)t;
   }
   __device__ __forceinline__ uint32_t of(int t) const {
     return BITS == 16 ? words[t >> 1] >> 16 * (t & 1) & 0xffffu : words[t];
-  }
-  // Whether any of the N tokens from t on (a multiple of N) occurs.
-  template <int N>
-  __device__ __forceinline__ bool any(int t) const {
-    constexpr int kBytes = N * BITS / 8;
-    const char* p = (const char*)words + t * (BITS / 8);
-    uint32_t w = 0;
-    if (kBytes == 8) {
-      const uint2 a = *reinterpret_cast<const uint2*>(p);
-      w = a.x | a.y;
-    } else {
-#pragma unroll
-      for (int i = 0; i < kBytes / 16; ++i) {
-        const uint4 a = reinterpret_cast<const uint4*>(p)[i];
-        w |= a.x | a.y | a.z | a.w;
-      }
-    }
-    return w != 0;
   }
 };
 
@@ -195,7 +182,10 @@ __global__ void __launch_bounds__(kProcThreads, 4) process_kernel(const __grid_c
   const int shift = rows::shift_of(in);
   const Slice<VE> slice(part, a.vps, shift, a.vocab);
   const RowMask mask = row_mask(a.r, row, a.status, threadIdx.x == 0 && part == 0);
-  Counters<BITS> counters{reinterpret_cast<uint32_t*>(slots)};  // token t at t - slice.first
+  __shared__ int listed;
+  // token t of the row is token t - slice.first here
+  const Counters<BITS> counters{reinterpret_cast<uint32_t*>(slots),
+                                reinterpret_cast<uint16_t*>((char*)slots + Counters<BITS>::count_bytes(a.vps * VE)), &listed};
   Penalties pen;
 
   if (HIST) {
@@ -240,58 +230,50 @@ __global__ void __launch_bounds__(kProcThreads, 4) process_kernel(const __grid_c
       if (t >= slice.lo && t < slice.hi) repeats.mark(t);
     }
   }
-  if (HIST || BIAS) __syncthreads();
 
   const bool lines_up = rows::lines_up(out, shift);
-  // the vector at e0 (the slice's vector i): penalties, mask, store
-  auto finish = [&](float* x, int i, int e0, uint32_t in_row, uint32_t ok, bool counted) {
-    if (HIST && counted) {
-#pragma unroll
-      for (int j = 0; j < VE; ++j)
-        // in place, a biased token keeps its logit: the bias pass takes it from there
-        if ((ok >> j & 1) && !(BIAS && a.in_place && repeats.listed(e0 + j)))
-          x[j] = pen.apply<BITS>(x[j], counters.of(i * VE + j));
-    }
-    if (ok != rows::kFull<VE>) {
-#pragma unroll
-      for (int j = 0; j < VE; ++j)
-        if (!(ok >> j & 1)) x[j] = kNegInf;
-    }
-    rows::store<TO, VE>(out, e0, in_row, lines_up, x);
-  };
-  slice.template each<kProcAhead>([&](int i, int e0, auto n) {
+  slice.template each<kProcAhead>([&](int, int e0, auto n) {
     constexpr int N = decltype(n)::value;
     uint4 raw[N];
     uint32_t ok[N];
-    bool counted[N], skip[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int e = e0 + j * stride * VE;
       ok[j] = mask.dead ? 0 : mask.words ? rows::allowed_whole<VE>(mask.words, e) : rows::kFull<VE>;
-      counted[j] = HIST && counters.template any<VE>((i + j * stride) * VE);
-      skip[j] = a.in_place && ok[j] == rows::kFull<VE> && !counted[j];  // nothing changes
       raw[j] = make_uint4(0, 0, 0, 0);
-      if (ok[j] && !skip[j]) raw[j] = rows::load16(in + e);
+      if (ok[j] && !(a.in_place && ok[j] == rows::kFull<VE>)) raw[j] = rows::load16(in + e);
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      if (skip[j]) continue;
+      if (a.in_place && ok[j] == rows::kFull<VE>) continue;  // nothing changes
       const int e = e0 + j * stride * VE;
-      float x[VE];
-      Vec<TI>::unpack(raw[j], x);
-      finish(x, i + j * stride, e, rows::kFull<VE>, ok[j], counted[j]);
+      if (ok[j] != rows::kFull<VE>) raw[j] = Vec<TI>::only(raw[j], ok[j]);
+      if (sizeof(TI) == sizeof(TO) && lines_up) {
+        *reinterpret_cast<uint4*>(out + e) = raw[j];
+      } else {
+        float x[VE];
+        Vec<TI>::unpack(raw[j], x);
+        rows::store<TO, VE>(out, e, rows::kFull<VE>, lines_up, x);
+      }
     }
   });
   slice.edges([&](int e0) {
     const uint32_t in_row = rows::inside<VE>(e0, a.vocab);
     const uint32_t ok = mask.dead ? 0 : mask.words ? rows::allowed<VE>(mask.words, e0, a.vocab) : in_row;
     float x[VE];
-    Vec<TI>::unpack(rows::load_raw(in, e0, in_row, ok), x);
-    finish(x, (e0 - slice.first) / VE, e0, in_row, ok, true);
+    Vec<TI>::unpack(Vec<TI>::only(rows::load_raw(in, e0, in_row, ok), ok), x);
+    rows::store<TO, VE>(out, e0, in_row, false, x);
   });
 
+  if (HIST || BIAS) __syncthreads();
+  if (HIST) {
+    for (int i = threadIdx.x; i < listed; i += stride) {
+      const int at = counters.list[i], t = slice.first + at;
+      if (!token_ok(mask, t) || (BIAS && repeats.listed(t))) continue;  // a biased token: below
+      out[t] = Vec<TO>::down(pen.apply<BITS>(Vec<TI>::up(in[t]), counters.of(at)));
+    }
+  }
   if (BIAS) {
-    __syncthreads();
     for (int64_t k = threadIdx.x; k < a.r.bias_count; k += stride) {
       const int t = __ldg(btok + k);
       if (t < slice.lo || t >= slice.hi || !token_ok(mask, t)) continue;
@@ -320,9 +302,12 @@ int launch_process(ProcArgs& a, int64_t n_rows, int64_t nv, cudaStream_t s) {
   const int64_t vps = std::min<int64_t>(nv, Repeats::kWords * 32 / VE);
   a.vps = (int)vps;
   a.split = (int)((nv + vps - 1) / vps);
-  const size_t smem = align_up((size_t)vps * VE * HIST / 8, 16);
+  const size_t smem = HIST ? Counters<HIST ? HIST : 32>::count_bytes(vps * VE) + 2 * std::min(vps * VE, a.r.history_len) : 0;
   const int threads = (int)std::min<int64_t>(kProcThreads, std::max<int64_t>(1, vps / (kProcAhead * 32)) * 32);
   if (n_rows * a.split > 0x7fffffff) return set_error(CNNUE_ERR_INVALID_ARG, "too many rows for one call");
+  if (smem > 40 * 1024)
+    CNNUE_CUDA_TRY(cudaFuncSetAttribute(process_kernel<TI, TO, HIST, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)smem));
   process_kernel<TI, TO, HIST, BIAS><<<(unsigned)(n_rows * a.split), threads, smem, s>>>(a);
   return check_launch_error("process_kernel");
 }

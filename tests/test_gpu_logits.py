@@ -229,16 +229,18 @@ def test_process_empty():
     assert torch.equal(out, x)
 
 
-def test_process_long_history_and_large_vocabulary():
-    R, V, L = 3, 200_003, 20_000
+@pytest.mark.parametrize("L", [20_000, 32_767, 32_768, 60_000])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_process_long_history_and_large_vocabulary(dtype, L):
+    R, V = 3, 100_003
     g = gen(9)
-    x = rows(R, V, torch.bfloat16, g)
+    x = rows(R, V, dtype, g)
     kw = dict(history=history_of(R, V, L, g), frequency=torch.rand(R, generator=g), repetition=1 + torch.rand(R, generator=g),
-              prompt_lengths=torch.tensor([0, 10_000, 20_000], dtype=torch.int32),
+              prompt_lengths=torch.tensor([0, 10_000, L], dtype=torch.int32),
               bias_tokens=torch.randint(0, V, (R, 300), generator=g).int(), bias_values=torch.randn(R, 300, generator=g),
               mask=mask_of(R, V, 0.9, g))
     want, bound = ref.process(x, **kw)
-    ref.close(lg.process_logits(dev(x), **{k: dev(t) for k, t in kw.items()}), want, bound, torch.bfloat16)
+    ref.close(lg.process_logits(dev(x), **{k: dev(t) for k, t in kw.items()}), want, bound, dtype)
 
 
 def test_process_captured_and_replayed_on_new_data():
