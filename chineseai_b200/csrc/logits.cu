@@ -80,10 +80,10 @@ struct Slice {
 };
 
 // Which of a list's tokens may occur in it more than once: a token's bit (by
-// its low 13 bits) is set a second time.  Tokens that share a bit by chance
+// its low 14 bits) is set a second time.  Tokens that share a bit by chance
 // are marked too, which costs time, not results.
 struct Repeats {
-  static constexpr int kWords = 256;
+  static constexpr int kWords = 512;
   uint32_t once[kWords], more[kWords];
   __device__ __forceinline__ void clear() {
     for (int i = threadIdx.x; i < kWords; i += blockDim.x) once[i] = more[i] = 0;
@@ -118,7 +118,9 @@ struct Repeats {
 // ---------------------------------------------------------------------------
 
 constexpr int kProcThreads = 256;
-constexpr int kProcAhead = 4;  // vectors per thread in flight
+constexpr int kProcAhead = 4;    // vectors per thread in flight
+constexpr int kTokensAhead = 4;  // history tokens per thread that are read before the slice is streamed,
+constexpr int kMoreTokens = 8;   // and after that, in flight
 
 struct ProcArgs {
   const void* in;
@@ -145,11 +147,43 @@ struct Counters {
       reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
     if (threadIdx.x == 0) *listed = 0;
   }
-  __device__ __forceinline__ void see(int t, bool prompt) const {
-    const int at = BITS == 16 ? 16 * (t & 1) : 0;
-    uint32_t* w = words + (BITS == 16 ? t >> 1 : t);
-    const uint32_t before = prompt ? atomicOr(w, kSeen << at) : atomicAdd(w, 1u << at);
-    if ((BITS == 16 ? before >> at & 0xffffu : before) == 0) list[atomicAdd(listed, 1)] = (uint16_t)t;
+  // Counts tokens t[0..N) (negative: none) at positions i, i + stride, ..; bit
+  // j of the result: t[j] had not occurred.  All atomics are under way before
+  // the first result is looked at.
+  template <int N>
+  __device__ __forceinline__ uint32_t see(const int* t, int64_t i, int stride, int64_t prompt) const {
+    uint32_t before[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int at = BITS == 16 ? 16 * (t[j] & 1) : 0;
+      uint32_t* w = words + (BITS == 16 ? t[j] >> 1 : t[j]);
+      const bool said = i + j * stride >= prompt;
+      before[j] = ~0u;
+      if (t[j] >= 0 && said) before[j] = atomicAdd(w, 1u << at);
+      if (t[j] >= 0 && !said) before[j] = atomicOr(w, kSeen << at);
+    }
+    uint32_t first = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (t[j] >= 0 && (BITS == 16 ? before[j] >> 16 * (t[j] & 1) & 0xffffu : before[j]) == 0) first |= 1u << j;
+    return first;
+  }
+  // The tokens t[j] that `which` names to the list; called by whole warps.
+  template <int N>
+  __device__ __forceinline__ void note(const int* t, uint32_t which) const {
+    const int lane = threadIdx.x & 31, n = __popc(which);
+    int at = n;  // inclusive sums over the warp
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int v = __shfl_up_sync(~0u, at, o);
+      if (lane >= o) at += v;
+    }
+    int base = 0;
+    if (lane == 31 && at > 0) base = atomicAdd(listed, at);
+    at += __shfl_sync(~0u, base, 31) - n;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (which >> j & 1) list[at++] = (uint16_t)t[j];
   }
   __device__ __forceinline__ uint32_t of(int t) const {
     return BITS == 16 ? words[t >> 1] >> 16 * (t & 1) & 0xffffu : words[t];
@@ -188,47 +222,33 @@ __global__ void __launch_bounds__(kProcThreads, 4) process_kernel(const __grid_c
                                 reinterpret_cast<uint16_t*>((char*)slots + Counters<BITS>::count_bytes(a.vps * VE)), &listed};
   Penalties pen;
 
+  // What the penalties and biases need is under way while the slice is
+  // streamed: nothing here waits for another load.
+  int64_t len = 0, prompt = 0;
+  const bool wide = a.r.history_bytes == 8;
+  const char* list = (const char*)a.r.history + row * a.r.history_stride * a.r.history_bytes;
+  int ahead[kTokensAhead];
+  auto read_tokens = [&](int64_t i, int64_t end) {
+#pragma unroll
+    for (int j = 0; j < kTokensAhead; ++j) ahead[j] = i + j * stride < end ? rows::token_at(list, i + j * stride, wide) : -1;
+  };
   if (HIST) {
-    counters.clear(slice.n * VE);
+    read_tokens(threadIdx.x, a.r.history_len);
+    len = a.r.lengths ? (int64_t)a.r.lengths[row] : a.r.history_len;
+    if (a.r.prompt_lengths) prompt = a.r.prompt_lengths[row];
     if (a.r.repetition) pen.rep = a.r.repetition[row];
     if (a.r.frequency) pen.freq = a.r.frequency[row];
     if (a.r.presence) pen.pres = a.r.presence[row];
-    int64_t len = a.r.history_len;
-    if (a.r.lengths) {
-      const int64_t l = a.r.lengths[row];
-      if ((l < 0 || l > len) && threadIdx.x == 0 && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_OFFSETS);
-      len = max((int64_t)0, min(l, len));
-    }
-    const int64_t prompt = a.r.prompt_lengths ? a.r.prompt_lengths[row] : 0;
-    const bool wide = a.r.history_bytes == 8;
-    const char* list = (const char*)a.r.history + row * a.r.history_stride * a.r.history_bytes;
-    bool bad = false;
-    __syncthreads();
-    for (int64_t i = threadIdx.x; i < len; i += 4 * stride) {
-      int t[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        t[j] = i + j * stride < len ? rows::token_at(list, i + j * stride, wide) : -1;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        bad |= t[j] >= a.vocab;
-        if (t[j] >= slice.lo && t[j] < slice.hi) counters.see(t[j] - slice.first, i + j * stride < prompt);
-      }
-    }
-    if (bad && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_INDEX);
+    counters.clear(slice.n * VE);
   }
   const int32_t* btok = nullptr;
   const float* bval = nullptr;
+  int biased = -1;  // entry threadIdx.x of the bias list
   if (BIAS) {
     btok = a.r.bias_tokens + row * a.r.bias_tokens_stride;
     bval = a.r.bias_values + row * a.r.bias_values_stride;
+    if (threadIdx.x < a.r.bias_count) biased = __ldg(btok + threadIdx.x);
     repeats.clear();
-    __syncthreads();
-    for (int64_t k = threadIdx.x; k < a.r.bias_count; k += stride) {
-      const int t = __ldg(btok + k);
-      if (t >= a.vocab && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_INDEX);
-      if (t >= slice.lo && t < slice.hi) repeats.mark(t);
-    }
   }
 
   const bool lines_up = rows::lines_up(out, shift);
@@ -265,32 +285,107 @@ __global__ void __launch_bounds__(kProcThreads, 4) process_kernel(const __grid_c
     rows::store<TO, VE>(out, e0, in_row, false, x);
   });
 
-  if (HIST || BIAS) __syncthreads();
+  if (!HIST && !BIAS) return;
+  auto value = [&](int t) { return Vec<TI>::up(in[t]); };  // streamed just now: from L2
+  // The first tokens' logits come while the counters are filled; of a token's
+  // occurrences the one that found its counter at 0 computes it.
+  float x[kTokensAhead];
+  uint32_t mine = 0, stays = 0;  // bit j: token j is this thread's to compute; the mask allows it
+  bool bad = false;
   if (HIST) {
-    for (int i = threadIdx.x; i < listed; i += stride) {
-      const int at = counters.list[i], t = slice.first + at;
-      if (!token_ok(mask, t) || (BIAS && repeats.listed(t))) continue;  // a biased token: below
-      out[t] = Vec<TO>::down(pen.apply<BITS>(Vec<TI>::up(in[t]), counters.of(at)));
+    if (len < 0 || len > a.r.history_len) {
+      if (threadIdx.x == 0 && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_OFFSETS);
+      len = max((int64_t)0, min(len, a.r.history_len));
+    }
+#pragma unroll
+    for (int j = 0; j < kTokensAhead; ++j) {
+      if (threadIdx.x + j * stride >= len) ahead[j] = -1;
+      bad |= ahead[j] >= a.vocab;
+      if (ahead[j] < slice.lo || ahead[j] >= slice.hi) ahead[j] = -1;
+      x[j] = ahead[j] >= 0 ? value(ahead[j]) : 0.f;
+      if (ahead[j] >= 0 && token_ok(mask, ahead[j])) stays |= 1u << j;
+    }
+  }
+  float x_biased = 0.f;
+  if (BIAS) {
+    bad |= biased >= a.vocab;
+    if (biased < slice.lo || biased >= slice.hi || !token_ok(mask, biased)) biased = -1;
+    if (biased >= 0) x_biased = value(biased);
+  }
+  __syncthreads();  // cleared
+  if (HIST) {
+    int at[kTokensAhead];
+#pragma unroll
+    for (int j = 0; j < kTokensAhead; ++j) at[j] = ahead[j] >= 0 ? ahead[j] - slice.first : -1;
+    mine = counters.template see<kTokensAhead>(at, threadIdx.x, stride, prompt);
+    for (int64_t b = kTokensAhead * stride; b < len; b += kMoreTokens * stride) {  // the same for all threads
+      const int64_t i = b + threadIdx.x;
+      int more[kMoreTokens];
+#pragma unroll
+      for (int j = 0; j < kMoreTokens; ++j)
+        more[j] = i + j * stride < len ? rows::token_at(list, i + j * stride, wide) : -1;
+#pragma unroll
+      for (int j = 0; j < kMoreTokens; ++j) {
+        bad |= more[j] >= a.vocab;
+        more[j] = more[j] >= slice.lo && more[j] < slice.hi ? more[j] - slice.first : -1;
+      }
+      const uint32_t first = counters.template see<kMoreTokens>(more, i, stride, prompt);
+      counters.template note<kMoreTokens>(more, first);
     }
   }
   if (BIAS) {
-    for (int64_t k = threadIdx.x; k < a.r.bias_count; k += stride) {
+    if (biased >= 0) repeats.mark(biased);
+    for (int64_t k = threadIdx.x + stride; k < a.r.bias_count; k += stride) {
       const int t = __ldg(btok + k);
-      if (t < slice.lo || t >= slice.hi || !token_ok(mask, t)) continue;
-      float x = Vec<TI>::up(in[t]);
-      if (HIST) x = pen.apply<BITS>(x, counters.of(t - slice.first));
+      bad |= t >= a.vocab;
+      if (t >= slice.lo && t < slice.hi && token_ok(mask, t)) repeats.mark(t);
+    }
+  }
+  if (bad && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_INDEX);
+  __syncthreads();
+  if (HIST) {  // a biased token: below
+#pragma unroll
+    for (int j = 0; j < kTokensAhead; ++j) {
+      if (!(mine & stays & 1u << j) || (BIAS && repeats.listed(ahead[j]))) continue;
+      out[ahead[j]] = Vec<TO>::down(pen.apply<BITS>(x[j], counters.of(ahead[j] - slice.first)));
+    }
+    const int n = listed;
+    for (int i = threadIdx.x; i < n; i += kTokensAhead * stride) {
+      int at[kTokensAhead];
+#pragma unroll
+      for (int j = 0; j < kTokensAhead; ++j) {
+        at[j] = i + j * stride < n ? counters.list[i + j * stride] : -1;
+        if (at[j] < 0) continue;
+        x[j] = value(slice.first + at[j]);
+        if (!token_ok(mask, slice.first + at[j]) || (BIAS && repeats.listed(slice.first + at[j]))) at[j] = -1;
+      }
+#pragma unroll
+      for (int j = 0; j < kTokensAhead; ++j)
+        if (at[j] >= 0) out[slice.first + at[j]] = Vec<TO>::down(pen.apply<BITS>(x[j], counters.of(at[j])));
+    }
+  }
+  if (BIAS) {
+    auto bias = [&](int64_t k, int t, float y) {
+      if (HIST) y = pen.apply<BITS>(y, counters.of(t - slice.first));
       if (!repeats.marked(t)) {
-        x = __fadd_rn(x, __ldg(bval + k));
+        y = __fadd_rn(y, __ldg(bval + k));
       } else {  // in list order, by the thread of the token's first entry
         bool earlier = false;
         for (int64_t j = 0; j < a.r.bias_count; ++j) {
           if (__ldg(btok + j) != t) continue;
           earlier |= j < k;
-          x = __fadd_rn(x, __ldg(bval + j));
+          y = __fadd_rn(y, __ldg(bval + j));
         }
-        if (earlier) continue;
+        if (earlier) return;
       }
-      out[t] = Vec<TO>::down(x);
+      out[t] = Vec<TO>::down(y);
+    };
+    if (biased >= 0) bias(threadIdx.x, biased, x_biased);
+    for (int64_t k = threadIdx.x + stride; k < a.r.bias_count; k += stride) {
+      const int t = __ldg(btok + k);
+      if (t < slice.lo || t >= slice.hi || !token_ok(mask, t)) continue;
+      // in place, a later entry of this token finds it written, and leaves it: it is marked
+      bias(k, t, value(t));
     }
   }
 }
@@ -298,17 +393,18 @@ __global__ void __launch_bounds__(kProcThreads, 4) process_kernel(const __grid_c
 template <typename TI, typename TO, int HIST, bool BIAS>
 int launch_process(ProcArgs& a, int64_t n_rows, int64_t nv, cudaStream_t s) {
   constexpr int VE = Vec<TI>::VE;
-  // At most 32 KB of counters; the bits of Repeats stand for one token each.
+  // At most 64 KB of counters; the bits of Repeats stand for one token each.
   const int64_t vps = std::min<int64_t>(nv, Repeats::kWords * 32 / VE);
   a.vps = (int)vps;
   a.split = (int)((nv + vps - 1) / vps);
-  const size_t smem = HIST ? Counters<HIST ? HIST : 32>::count_bytes(vps * VE) + 2 * std::min(vps * VE, a.r.history_len) : 0;
-  const int threads = (int)std::min<int64_t>(kProcThreads, std::max<int64_t>(1, vps / (kProcAhead * 32)) * 32);
   if (n_rows * a.split > 0x7fffffff) return set_error(CNNUE_ERR_INVALID_ARG, "too many rows for one call");
+  auto* kernel = process_kernel<TI, TO, HIST, BIAS>;
+  const int threads = (int)std::min<int64_t>(kProcThreads, std::max<int64_t>(1, vps / (kProcAhead * 32)) * 32);
+  size_t smem = 0;
+  if (HIST) smem = Counters<HIST ? HIST : 32>::count_bytes(vps * VE) + 2 * std::min(vps * VE, a.r.history_len);
   if (smem > 40 * 1024)
-    CNNUE_CUDA_TRY(cudaFuncSetAttribute(process_kernel<TI, TO, HIST, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)smem));
-  process_kernel<TI, TO, HIST, BIAS><<<(unsigned)(n_rows * a.split), threads, smem, s>>>(a);
+    CNNUE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  kernel<<<(unsigned)(n_rows * a.split), threads, smem, s>>>(a);
   return check_launch_error("process_kernel");
 }
 
