@@ -80,10 +80,10 @@ struct Slice {
 };
 
 // Which of a list's tokens may occur in it more than once: a token's bit (by
-// its low 14 bits) is set a second time.  Tokens that share a bit by chance
+// its low 13 bits) is set a second time.  Tokens that share a bit by chance
 // are marked too, which costs time, not results.
 struct Repeats {
-  static constexpr int kWords = 512;
+  static constexpr int kWords = 256;
   uint32_t once[kWords], more[kWords];
   __device__ __forceinline__ void clear() {
     for (int i = threadIdx.x; i < kWords; i += blockDim.x) once[i] = more[i] = 0;
@@ -92,7 +92,6 @@ struct Repeats {
     const uint32_t word = (uint32_t)tok / 32 % kWords, bit = 1u << (tok & 31);
     if (atomicOr(once + word, bit) & bit) atomicOr(more + word, bit);
   }
-  __device__ __forceinline__ bool listed(int tok) const { return once[(uint32_t)tok / 32 % kWords] >> (tok & 31) & 1; }
   __device__ __forceinline__ bool marked(int tok) const { return more[(uint32_t)tok / 32 % kWords] >> (tok & 31) & 1; }
 };
 
@@ -106,151 +105,48 @@ struct Repeats {
 //   x = x + bias            for the token's biases in list order
 //   not allowed:           x = -inf
 //
-// Every step is one IEEE fp32 operation.  A CTA takes one slice of one row.
-// It counts the history's tokens that fall into the slice in shared memory
-// (integer atomics: their order does not change the counts) and notes each
-// token's first occurrence in a list; it streams the slice through the mask
-// (what that excludes is not read); and after a barrier it computes the listed
-// tokens, whose logits are in L2 by then, and the biased ones, and stores them
-// over.  With the counters looked up for every vector on its way instead, most
-// warps held some penalised token and went the slow way: 253 us for 2048 x
-// 50001 fp16 with 512 tokens of history.
+// Every step is one IEEE fp32 operation.  Two parts: the rows are streamed
+// through the mask (what that excludes is not read), and the tokens that are
+// penalised or biased, a few hundred or thousand of a row, are computed from
+// their logits, which are in L2 by then, and stored over.  The second part
+// needs to know how often a token occurs: shared memory counts it, by integer
+// atomics (their order does not change the counts), and the occurrence that
+// found the counter at 0 computes the token.
+//
+// A row of up to kFusedTokens tokens is one CTA's, both parts in one launch.
+// Longer rows are streamed by as many CTAs as they need and the second part is
+// a launch of its own, whose reading and counting overlap the streaming
+// (programmatic dependent launch).  With the counting in every slice's CTA
+// instead, each read the whole history and had few threads left to stream:
+// 135 us for 2048 x 50001 fp16 with 512 tokens of history, 37 us for 64 x
+// 131072 bf16 with 8192.
 // ---------------------------------------------------------------------------
 
 constexpr int kProcThreads = 256;
-constexpr int kProcAhead = 4;    // vectors per thread in flight
-constexpr int kTokensAhead = 4;  // history tokens per thread that are read before the slice is streamed,
-constexpr int kMoreTokens = 8;   // and after that, in flight
+constexpr int kProcAhead = 4;        // vectors per thread in flight
+constexpr int kFusedTokens = 16384;  // 32 or 64 KB of counters
+constexpr int kCountThreads = 512;
+constexpr int kTokensAhead = 4;  // history tokens per thread that are read first of all,
+constexpr int kMoreTokens = 8;   // and after those, in flight
+constexpr int kHashTokens = kCountThreads * kTokensAhead;  // the longest history that is counted in a hash table
 
 struct ProcArgs {
   const void* in;
   void* out;
   int64_t in_stride, out_stride;
-  int vocab, split, vps;  // slices per row, vectors per slice
+  int vocab, split, vps;  // streaming: slices per row, vectors per slice
+  int slots, lg;          // counting: counters per CTA; 1 << lg CTAs per row
   bool in_place;
   cnnue_logit_rules r;
   uint32_t* status;
 };
 
-// Counters of BITS bits per token: the high bit says that the token occurs,
-// the others how often after the prompt.  16 bits hold the counts of histories
-// of up to 32767 tokens.  Then the list of the tokens that occur, in no order.
-template <int BITS>
-struct Counters {
-  static constexpr uint32_t kSeen = 1u << (BITS - 1);
-  uint32_t* words;
-  uint16_t* list;
-  int* listed;
-  static __host__ __device__ int64_t count_bytes(int64_t tokens) { return (tokens * BITS / 8 + 15) / 16 * 16; }
-  __device__ __forceinline__ void clear(int tokens) const {
-    for (int i = threadIdx.x; i < count_bytes(tokens) / 16; i += blockDim.x)
-      reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x == 0) *listed = 0;
-  }
-  // Counts tokens t[0..N) (negative: none) at positions i, i + stride, ..; bit
-  // j of the result: t[j] had not occurred.  All atomics are under way before
-  // the first result is looked at.
-  template <int N>
-  __device__ __forceinline__ uint32_t see(const int* t, int64_t i, int stride, int64_t prompt) const {
-    uint32_t before[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int at = BITS == 16 ? 16 * (t[j] & 1) : 0;
-      uint32_t* w = words + (BITS == 16 ? t[j] >> 1 : t[j]);
-      const bool said = i + j * stride >= prompt;
-      before[j] = ~0u;
-      if (t[j] >= 0 && said) before[j] = atomicAdd(w, 1u << at);
-      if (t[j] >= 0 && !said) before[j] = atomicOr(w, kSeen << at);
-    }
-    uint32_t first = 0;
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (t[j] >= 0 && (BITS == 16 ? before[j] >> 16 * (t[j] & 1) & 0xffffu : before[j]) == 0) first |= 1u << j;
-    return first;
-  }
-  // The tokens t[j] that `which` names to the list; called by whole warps.
-  template <int N>
-  __device__ __forceinline__ void note(const int* t, uint32_t which) const {
-    const int lane = threadIdx.x & 31, n = __popc(which);
-    int at = n;  // inclusive sums over the warp
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-      const int v = __shfl_up_sync(~0u, at, o);
-      if (lane >= o) at += v;
-    }
-    int base = 0;
-    if (lane == 31 && at > 0) base = atomicAdd(listed, at);
-    at += __shfl_sync(~0u, base, 31) - n;
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (which >> j & 1) list[at++] = (uint16_t)t[j];
-  }
-  __device__ __forceinline__ uint32_t of(int t) const {
-    return BITS == 16 ? words[t >> 1] >> 16 * (t & 1) & 0xffffu : words[t];
-  }
-};
-
-struct Penalties {
-  float rep = 1.f, freq = 0.f, pres = 0.f;
-  // `c`: a counter without its high bit's place, 0 = the token does not occur.
-  template <int BITS>
-  __device__ __forceinline__ float apply(float x, uint32_t c) const {
-    if (c == 0) return x;
-    x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-    const uint32_t n = c & ~Counters<BITS>::kSeen;
-    return n ? __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)n)), pres) : x;
-  }
-};
-
-// HIST: 0, or the counters' bits.
-template <typename TI, typename TO, int HIST, bool BIAS>
-__global__ void __launch_bounds__(kProcThreads, 4) process_kernel(const __grid_constant__ ProcArgs a) {
+// Streams one slice of a row through the mask.
+template <typename TI, typename TO>
+__device__ __forceinline__ void stream_slice(const ProcArgs& a, const TI* in, TO* out, int part, const RowMask& mask) {
   constexpr int VE = Vec<TI>::VE;
-  constexpr int BITS = HIST ? HIST : 32;
-  extern __shared__ uint4 slots[];
-  __shared__ Repeats repeats;
-  const int64_t row = blockIdx.x / a.split;
-  const int part = (int)(blockIdx.x % a.split), stride = blockDim.x;
-  const TI* in = (const TI*)a.in + row * a.in_stride;
-  TO* out = (TO*)a.out + row * a.out_stride;
-  const int shift = rows::shift_of(in);
+  const int shift = rows::shift_of(in), stride = blockDim.x;
   const Slice<VE> slice(part, a.vps, shift, a.vocab);
-  const RowMask mask = row_mask(a.r, row, a.status, threadIdx.x == 0 && part == 0);
-  __shared__ int listed;
-  // token t of the row is token t - slice.first here
-  const Counters<BITS> counters{reinterpret_cast<uint32_t*>(slots),
-                                reinterpret_cast<uint16_t*>((char*)slots + Counters<BITS>::count_bytes(a.vps * VE)), &listed};
-  Penalties pen;
-
-  // What the penalties and biases need is under way while the slice is
-  // streamed: nothing here waits for another load.
-  int64_t len = 0, prompt = 0;
-  const bool wide = a.r.history_bytes == 8;
-  const char* list = (const char*)a.r.history + row * a.r.history_stride * a.r.history_bytes;
-  int ahead[kTokensAhead];
-  auto read_tokens = [&](int64_t i, int64_t end) {
-#pragma unroll
-    for (int j = 0; j < kTokensAhead; ++j) ahead[j] = i + j * stride < end ? rows::token_at(list, i + j * stride, wide) : -1;
-  };
-  if (HIST) {
-    read_tokens(threadIdx.x, a.r.history_len);
-    len = a.r.lengths ? (int64_t)a.r.lengths[row] : a.r.history_len;
-    if (a.r.prompt_lengths) prompt = a.r.prompt_lengths[row];
-    if (a.r.repetition) pen.rep = a.r.repetition[row];
-    if (a.r.frequency) pen.freq = a.r.frequency[row];
-    if (a.r.presence) pen.pres = a.r.presence[row];
-    counters.clear(slice.n * VE);
-  }
-  const int32_t* btok = nullptr;
-  const float* bval = nullptr;
-  int biased = -1;  // entry threadIdx.x of the bias list
-  if (BIAS) {
-    btok = a.r.bias_tokens + row * a.r.bias_tokens_stride;
-    bval = a.r.bias_values + row * a.r.bias_values_stride;
-    if (threadIdx.x < a.r.bias_count) biased = __ldg(btok + threadIdx.x);
-    repeats.clear();
-  }
-
   const bool lines_up = rows::lines_up(out, shift);
   slice.template each<kProcAhead>([&](int, int e0, auto n) {
     constexpr int N = decltype(n)::value;
@@ -284,128 +180,294 @@ __global__ void __launch_bounds__(kProcThreads, 4) process_kernel(const __grid_c
     Vec<TI>::unpack(Vec<TI>::only(rows::load_raw(in, e0, in_row, ok), ok), x);
     rows::store<TO, VE>(out, e0, in_row, false, x);
   });
+}
 
-  if (!HIST && !BIAS) return;
-  auto value = [&](int t) { return Vec<TI>::up(in[t]); };  // streamed just now: from L2
-  // The first tokens' logits come while the counters are filled; of a token's
-  // occurrences the one that found its counter at 0 computes it.
-  float x[kTokensAhead];
-  uint32_t mine = 0, stays = 0;  // bit j: token j is this thread's to compute; the mask allows it
+// What a CTA knows of its tokens, in shared memory: a slot per token, with a
+// counter of BITS bits (the high bit says that the token occurs, the others
+// how often after the prompt; 16 bits do for histories of up to 32767 tokens),
+// two bits for the bias list (named once, named again), and a list of slots.
+// HASH: the slots are a hash table of tokens, at most half full, for short
+// histories over any vocabulary; else CTA p of the row's 1 << lg owns the tokens
+// t with t mod (1 << lg) = p, token t in slot t >> lg (text uses low tokens
+// most: neighbours are dealt to different CTAs).
+template <int BITS, bool HASH>
+struct Table {
+  static constexpr uint32_t kSeen = 1u << (BITS - 1);
+  uint32_t *words, *keys, *once, *more;
+  uint16_t* list;
+  int* listed;
+  int slots, lg;
+
+  static __host__ __device__ size_t bytes(int64_t slots, bool bias, int64_t longest) {
+    return (size_t)((slots * BITS / 8 + 15) / 16 * 16 + (HASH ? slots * 4 : 0) + (bias ? (slots + 31) / 32 * 8 : 0) +
+                    (HASH ? 0 : 2 * (slots < longest ? slots : longest)) + 16);
+  }
+  __device__ __forceinline__ Table(void* smem, int* counter, int n, int log_ctas, bool bias)
+      : listed(counter), slots(n), lg(log_ctas) {
+    words = (uint32_t*)smem;
+    keys = words + (slots * BITS / 8 + 15) / 16 * 4;
+    once = keys + (HASH ? slots : 0);
+    more = once + (bias ? (slots + 31) / 32 : 0);
+    list = (uint16_t*)(more + (bias ? (slots + 31) / 32 : 0));
+  }
+  __device__ __forceinline__ void clear(bool bias) const {
+    for (int i = threadIdx.x; i < (slots * BITS / 8 + 15) / 16; i += blockDim.x)
+      reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+    if (HASH)
+      for (int i = threadIdx.x; i < slots; i += blockDim.x) keys[i] = ~0u;
+    if (bias)
+      for (int i = threadIdx.x; i < (slots + 31) / 32; i += blockDim.x) once[i] = more[i] = 0;
+    if (threadIdx.x == 0) *listed = 0;
+  }
+  // The slot of token t (the table holds it, or gets it).
+  __device__ __forceinline__ int slot(int t) const {
+    if (!HASH) return t >> lg;
+    uint32_t h = (uint32_t)t * 2654435761u >> __clz(slots - 1);
+    for (int n = 0; n < slots; ++n) {  // ends at a free slot: half of them are
+      const uint32_t k = atomicCAS(keys + h, ~0u, (uint32_t)t);
+      if (k == ~0u || k == (uint32_t)t) break;
+      h = (h + 1) & (slots - 1);
+    }
+    return (int)h;
+  }
+  __device__ __forceinline__ int token(int s, int part) const { return s << lg | part; }
+  // Counts the tokens in slots s[0..N) (negative: none) at positions i, i +
+  // stride, ..; bit j of the result: s[j] had not occurred.
+  template <int N>
+  __device__ __forceinline__ uint32_t see(const int* s, int64_t i, int stride, int64_t prompt) const {
+    uint32_t before[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int at = BITS == 16 ? 16 * (s[j] & 1) : 0;
+      uint32_t* w = words + (BITS == 16 ? s[j] >> 1 : s[j]);
+      const bool said = i + j * stride >= prompt;
+      before[j] = ~0u;
+      if (s[j] >= 0 && said) before[j] = atomicAdd(w, 1u << at);
+      if (s[j] >= 0 && !said) before[j] = atomicOr(w, kSeen << at);
+    }
+    uint32_t first = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (s[j] >= 0 && (BITS == 16 ? before[j] >> 16 * (s[j] & 1) & 0xffffu : before[j]) == 0) first |= 1u << j;
+    return first;
+  }
+  // The slots s[j] that `which` names to the list; called by whole warps.
+  template <int N>
+  __device__ __forceinline__ void note(const int* s, uint32_t which) const {
+    const int lane = threadIdx.x & 31, n = __popc(which);
+    int at = n;  // inclusive sums over the warp
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int v = __shfl_up_sync(~0u, at, o);
+      if (lane >= o) at += v;
+    }
+    int base = 0;
+    if (lane == 31 && at > 0) base = atomicAdd(listed, at);
+    at += __shfl_sync(~0u, base, 31) - n;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (which >> j & 1) list[at++] = (uint16_t)s[j];
+  }
+  __device__ __forceinline__ uint32_t count(int s) const {
+    return BITS == 16 ? words[s >> 1] >> 16 * (s & 1) & 0xffffu : words[s];
+  }
+  __device__ __forceinline__ void mark(int s) const {
+    const uint32_t bit = 1u << (s & 31);
+    if (atomicOr(once + (s >> 5), bit) & bit) atomicOr(more + (s >> 5), bit);
+  }
+  __device__ __forceinline__ bool biased(int s) const { return once[s >> 5] >> (s & 31) & 1; }
+  __device__ __forceinline__ bool again(int s) const { return more[s >> 5] >> (s & 31) & 1; }
+};
+
+struct Penalties {
+  float rep = 1.f, freq = 0.f, pres = 0.f;
+  // `c`: a counter, 0 = the token does not occur.
+  template <int BITS>
+  __device__ __forceinline__ float apply(float x, uint32_t c) const {
+    if (c == 0) return x;
+    x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+    const uint32_t n = c & ~(1u << (BITS - 1));
+    return n ? __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)n)), pres) : x;
+  }
+};
+
+// The penalised and biased tokens of a row that CTA `part` owns.  `streamed()`
+// is called before the first store, when the loads that need not wait for the
+// streamed row are under way.
+template <typename TI, typename TO, int BITS, bool HASH, typename F>
+__device__ __forceinline__ void penalise(const ProcArgs& a, const TI* in, TO* out, int64_t row, int part,
+                                         const RowMask& mask, void* smem, F&& streamed) {
+  __shared__ int listed;
+  const int stride = blockDim.x;
+  const bool hist = a.r.history != nullptr, bias = a.r.bias_tokens != nullptr;
+  const Table<BITS, HASH> table(smem, &listed, a.slots, a.lg, bias);
+  Penalties pen;
+  int64_t len = 0, prompt = 0;
+  const bool wide = a.r.history_bytes == 8;
+  const char* list = (const char*)a.r.history + row * a.r.history_stride * a.r.history_bytes;
+  int ahead[kTokensAhead];
+#pragma unroll
+  for (int j = 0; j < kTokensAhead; ++j) {
+    const int64_t i = threadIdx.x + j * stride;
+    ahead[j] = hist && i < a.r.history_len ? rows::token_at(list, i, wide) : -1;
+  }
+  if (hist) {
+    len = a.r.lengths ? (int64_t)a.r.lengths[row] : a.r.history_len;
+    if (a.r.prompt_lengths) prompt = a.r.prompt_lengths[row];
+    if (a.r.repetition) pen.rep = a.r.repetition[row];
+    if (a.r.frequency) pen.freq = a.r.frequency[row];
+    if (a.r.presence) pen.pres = a.r.presence[row];
+  }
+  const int32_t* btok = a.r.bias_tokens + row * a.r.bias_tokens_stride;
+  const float* bval = a.r.bias_values + row * a.r.bias_values_stride;
+  int biased = bias && threadIdx.x < a.r.bias_count ? __ldg(btok + threadIdx.x) : -1;
+  table.clear(bias);
+
   bool bad = false;
-  if (HIST) {
-    if (len < 0 || len > a.r.history_len) {
-      if (threadIdx.x == 0 && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_OFFSETS);
-      len = max((int64_t)0, min(len, a.r.history_len));
-    }
+  auto own = [&](int t) {  // t, or -1 if it is none of this CTA's tokens
+    bad |= t >= a.vocab;
+    return t >= 0 && t < a.vocab && (HASH || (t & ((1 << a.lg) - 1)) == part) ? t : -1;
+  };
+  auto value = [&](int t) { return Vec<TI>::up(in[t]); };
+  float x[kTokensAhead], x_biased = 0.f;
+  uint32_t mine = 0, stays = 0;  // bit j: token j is this thread's to compute; the mask allows it
+  if (len < 0 || len > a.r.history_len) {
+    if (hist && threadIdx.x == 0 && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_OFFSETS);
+    len = max((int64_t)0, min(len, a.r.history_len));
+  }
 #pragma unroll
-    for (int j = 0; j < kTokensAhead; ++j) {
-      if (threadIdx.x + j * stride >= len) ahead[j] = -1;
-      bad |= ahead[j] >= a.vocab;
-      if (ahead[j] < slice.lo || ahead[j] >= slice.hi) ahead[j] = -1;
-      x[j] = ahead[j] >= 0 ? value(ahead[j]) : 0.f;
-      if (ahead[j] >= 0 && token_ok(mask, ahead[j])) stays |= 1u << j;
-    }
+  for (int j = 0; j < kTokensAhead; ++j) {
+    ahead[j] = threadIdx.x + j * stride < len ? own(ahead[j]) : -1;
+    x[j] = ahead[j] >= 0 ? value(ahead[j]) : 0.f;
+    if (ahead[j] >= 0 && token_ok(mask, ahead[j])) stays |= 1u << j;
   }
-  float x_biased = 0.f;
-  if (BIAS) {
-    bad |= biased >= a.vocab;
-    if (biased < slice.lo || biased >= slice.hi || !token_ok(mask, biased)) biased = -1;
-    if (biased >= 0) x_biased = value(biased);
-  }
+  biased = own(biased);
+  if (biased >= 0 && !token_ok(mask, biased)) biased = -1;
+  if (biased >= 0) x_biased = value(biased);
   __syncthreads();  // cleared
-  if (HIST) {
-    int at[kTokensAhead];
+
+  int at[kTokensAhead], at_biased = -1;
 #pragma unroll
-    for (int j = 0; j < kTokensAhead; ++j) at[j] = ahead[j] >= 0 ? ahead[j] - slice.first : -1;
-    mine = counters.template see<kTokensAhead>(at, threadIdx.x, stride, prompt);
+  for (int j = 0; j < kTokensAhead; ++j) at[j] = ahead[j] >= 0 ? table.slot(ahead[j]) : -1;
+  mine = table.template see<kTokensAhead>(at, threadIdx.x, stride, prompt);
+  if (!HASH) {  // a hash table's histories end here
     for (int64_t b = kTokensAhead * stride; b < len; b += kMoreTokens * stride) {  // the same for all threads
       const int64_t i = b + threadIdx.x;
-      int more[kMoreTokens];
+      int s[kMoreTokens];
 #pragma unroll
-      for (int j = 0; j < kMoreTokens; ++j)
-        more[j] = i + j * stride < len ? rows::token_at(list, i + j * stride, wide) : -1;
+      for (int j = 0; j < kMoreTokens; ++j) s[j] = i + j * stride < len ? rows::token_at(list, i + j * stride, wide) : -1;
 #pragma unroll
-      for (int j = 0; j < kMoreTokens; ++j) {
-        bad |= more[j] >= a.vocab;
-        more[j] = more[j] >= slice.lo && more[j] < slice.hi ? more[j] - slice.first : -1;
-      }
-      const uint32_t first = counters.template see<kMoreTokens>(more, i, stride, prompt);
-      counters.template note<kMoreTokens>(more, first);
+      for (int j = 0; j < kMoreTokens; ++j) s[j] = own(s[j]) >= 0 ? table.slot(s[j]) : -1;
+      const uint32_t first = table.template see<kMoreTokens>(s, i, stride, prompt);
+      table.template note<kMoreTokens>(s, first);
     }
   }
-  if (BIAS) {
-    if (biased >= 0) repeats.mark(biased);
+  if (biased >= 0) table.mark(at_biased = table.slot(biased));
+  if (bias) {
     for (int64_t k = threadIdx.x + stride; k < a.r.bias_count; k += stride) {
-      const int t = __ldg(btok + k);
-      bad |= t >= a.vocab;
-      if (t >= slice.lo && t < slice.hi && token_ok(mask, t)) repeats.mark(t);
+      const int t = own(__ldg(btok + k));
+      if (t >= 0 && token_ok(mask, t)) table.mark(table.slot(t));
     }
   }
   if (bad && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_INDEX);
-  __syncthreads();
-  if (HIST) {  // a biased token: below
+  __syncthreads();  // counted
+  streamed();
+
 #pragma unroll
-    for (int j = 0; j < kTokensAhead; ++j) {
-      if (!(mine & stays & 1u << j) || (BIAS && repeats.listed(ahead[j]))) continue;
-      out[ahead[j]] = Vec<TO>::down(pen.apply<BITS>(x[j], counters.of(ahead[j] - slice.first)));
-    }
+  for (int j = 0; j < kTokensAhead; ++j)  // a biased token: below
+    if ((mine & stays & 1u << j) && !(bias && table.biased(at[j])))
+      out[ahead[j]] = Vec<TO>::down(pen.apply<BITS>(x[j], table.count(at[j])));
+  if (!HASH) {
     const int n = listed;
     for (int i = threadIdx.x; i < n; i += kTokensAhead * stride) {
-      int at[kTokensAhead];
+      int s[kTokensAhead], t[kTokensAhead];
 #pragma unroll
       for (int j = 0; j < kTokensAhead; ++j) {
-        at[j] = i + j * stride < n ? counters.list[i + j * stride] : -1;
-        if (at[j] < 0) continue;
-        x[j] = value(slice.first + at[j]);
-        if (!token_ok(mask, slice.first + at[j]) || (BIAS && repeats.listed(slice.first + at[j]))) at[j] = -1;
+        s[j] = i + j * stride < n ? table.list[i + j * stride] : -1;
+        if (s[j] < 0) continue;
+        t[j] = table.token(s[j], part);
+        x[j] = value(t[j]);
+        if (!token_ok(mask, t[j]) || (bias && table.biased(s[j]))) s[j] = -1;
       }
 #pragma unroll
       for (int j = 0; j < kTokensAhead; ++j)
-        if (at[j] >= 0) out[slice.first + at[j]] = Vec<TO>::down(pen.apply<BITS>(x[j], counters.of(at[j])));
+        if (s[j] >= 0) out[t[j]] = Vec<TO>::down(pen.apply<BITS>(x[j], table.count(s[j])));
     }
   }
-  if (BIAS) {
-    auto bias = [&](int64_t k, int t, float y) {
-      if (HIST) y = pen.apply<BITS>(y, counters.of(t - slice.first));
-      if (!repeats.marked(t)) {
-        y = __fadd_rn(y, __ldg(bval + k));
-      } else {  // in list order, by the thread of the token's first entry
-        bool earlier = false;
-        for (int64_t j = 0; j < a.r.bias_count; ++j) {
-          if (__ldg(btok + j) != t) continue;
-          earlier |= j < k;
-          y = __fadd_rn(y, __ldg(bval + j));
-        }
-        if (earlier) return;
+  auto add_bias = [&](int64_t k, int t, int s, float y) {
+    y = pen.apply<BITS>(y, table.count(s));
+    if (!table.again(s)) {
+      y = __fadd_rn(y, __ldg(bval + k));
+    } else {  // in list order, by the thread of the token's first entry
+      bool earlier = false;
+      for (int64_t j = 0; j < a.r.bias_count; ++j) {
+        if (__ldg(btok + j) != t) continue;
+        earlier |= j < k;
+        y = __fadd_rn(y, __ldg(bval + j));
       }
-      out[t] = Vec<TO>::down(y);
-    };
-    if (biased >= 0) bias(threadIdx.x, biased, x_biased);
+      if (earlier) return;
+    }
+    out[t] = Vec<TO>::down(y);
+  };
+  if (biased >= 0) add_bias(threadIdx.x, biased, at_biased, x_biased);
+  if (bias) {
     for (int64_t k = threadIdx.x + stride; k < a.r.bias_count; k += stride) {
-      const int t = __ldg(btok + k);
-      if (t < slice.lo || t >= slice.hi || !token_ok(mask, t)) continue;
-      // in place, a later entry of this token finds it written, and leaves it: it is marked
-      bias(k, t, value(t));
+      const int t = own(__ldg(btok + k));
+      // in place, a later entry of a token finds it written, and leaves it: its slot is marked
+      if (t >= 0 && token_ok(mask, t)) add_bias(k, t, table.slot(t), value(t));
     }
   }
 }
 
-template <typename TI, typename TO, int HIST, bool BIAS>
-int launch_process(ProcArgs& a, int64_t n_rows, int64_t nv, cudaStream_t s) {
-  constexpr int VE = Vec<TI>::VE;
-  // At most 64 KB of counters; the bits of Repeats stand for one token each.
-  const int64_t vps = std::min<int64_t>(nv, Repeats::kWords * 32 / VE);
-  a.vps = (int)vps;
-  a.split = (int)((nv + vps - 1) / vps);
-  if (n_rows * a.split > 0x7fffffff) return set_error(CNNUE_ERR_INVALID_ARG, "too many rows for one call");
-  auto* kernel = process_kernel<TI, TO, HIST, BIAS>;
-  const int threads = (int)std::min<int64_t>(kProcThreads, std::max<int64_t>(1, vps / (kProcAhead * 32)) * 32);
-  size_t smem = 0;
-  if (HIST) smem = Counters<HIST ? HIST : 32>::count_bytes(vps * VE) + 2 * std::min(vps * VE, a.r.history_len);
+template <typename TI, typename TO>
+__global__ void __launch_bounds__(kProcThreads, 8) stream_kernel(const __grid_constant__ ProcArgs a) {
+  const int64_t row = blockIdx.x / (unsigned)a.split;
+  const int part = (int)(blockIdx.x % (unsigned)a.split);
+  const RowMask mask = row_mask(a.r, row, a.status, threadIdx.x == 0 && part == 0);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  stream_slice<TI, TO>(a, (const TI*)a.in + row * a.in_stride, (TO*)a.out + row * a.out_stride, part, mask);
+}
+
+template <typename TI, typename TO, int BITS>
+__global__ void __launch_bounds__(kProcThreads, 4) fused_kernel(const __grid_constant__ ProcArgs a) {
+  extern __shared__ uint4 smem[];
+  const int64_t row = blockIdx.x;
+  const TI* in = (const TI*)a.in + row * a.in_stride;
+  TO* out = (TO*)a.out + row * a.out_stride;
+  const RowMask mask = row_mask(a.r, row, a.status, threadIdx.x == 0);
+  stream_slice<TI, TO>(a, in, out, 0, mask);
+  penalise<TI, TO, BITS, false>(a, in, out, row, 0, mask, smem, [] {});  // its barriers order the stores
+}
+
+template <typename TI, typename TO, int BITS, bool HASH>
+__global__ void __launch_bounds__(kCountThreads, 2) penalise_kernel(const __grid_constant__ ProcArgs a) {
+  extern __shared__ uint4 smem[];
+  const int64_t row = blockIdx.x >> a.lg;
+  const RowMask mask = row_mask(a.r, row, a.status, false);
+  // in place, streaming writes -inf to what the mask excludes: those logits are not used here
+  penalise<TI, TO, BITS, HASH>(a, (const TI*)a.in + row * a.in_stride, (TO*)a.out + row * a.out_stride, row,
+                               (int)(blockIdx.x & ((1u << a.lg) - 1)), mask, smem,
+                               [] { asm volatile("griddepcontrol.wait;" ::: "memory"); });
+}
+
+template <typename F>
+int launch_process(F* kernel, const ProcArgs& a, int64_t blocks, int threads, size_t smem, bool dependent, cudaStream_t s,
+                   const char* what) {
+  if (blocks > 0x7fffffff) return set_error(CNNUE_ERR_INVALID_ARG, "too many rows for one call");
   if (smem > 40 * 1024)
     CNNUE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kernel<<<(unsigned)(n_rows * a.split), threads, smem, s>>>(a);
-  return check_launch_error("process_kernel");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  CNNUE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
+  return check_launch_error(what);
 }
 
 // Vectors that cover a row: one more only where a row may start inside one.
@@ -418,12 +480,50 @@ int64_t row_vectors(const void* p, int64_t stride, int64_t vocab) {
 template <typename TI, typename TO>
 int pick_process(ProcArgs& a, int64_t n_rows, cudaStream_t s) {
   const int64_t nv = row_vectors<TI>(a.in, a.in_stride, a.vocab);
-  const bool hist = a.r.history && a.r.history_len > 0 && (a.r.repetition || a.r.frequency || a.r.presence);
-  const bool bias = a.r.bias_tokens && a.r.bias_count > 0;
-  if (!hist) return bias ? launch_process<TI, TO, 0, true>(a, n_rows, nv, s) : launch_process<TI, TO, 0, false>(a, n_rows, nv, s);
-  if (a.r.history_len < 32768)
-    return bias ? launch_process<TI, TO, 16, true>(a, n_rows, nv, s) : launch_process<TI, TO, 16, false>(a, n_rows, nv, s);
-  return bias ? launch_process<TI, TO, 32, true>(a, n_rows, nv, s) : launch_process<TI, TO, 32, false>(a, n_rows, nv, s);
+  if (!a.r.history || a.r.history_len == 0 || (!a.r.repetition && !a.r.frequency && !a.r.presence)) {
+    a.r.history = nullptr;
+    a.r.history_len = 0;
+  }
+  if (a.r.bias_count == 0) a.r.bias_tokens = nullptr;
+  const bool count = a.r.history || a.r.bias_tokens, bias = a.r.bias_tokens != nullptr, wide = a.r.history_len > 32767;
+  const int64_t len = a.r.history_len;
+  auto per_thread = [](int64_t n, int each, int most) {  // threads for n items
+    return (int)std::min<int64_t>(most, std::max<int64_t>(1, n / (each * 32)) * 32);
+  };
+  if (count && a.vocab <= kFusedTokens) {
+    a.split = 1, a.vps = (int)nv, a.slots = a.vocab, a.lg = 0;
+    const int threads = per_thread(nv, kProcAhead, kProcThreads);
+    return wide ? launch_process(fused_kernel<TI, TO, 32>, a, n_rows, threads,
+                                 Table<32, false>::bytes(a.slots, bias, len), false, s, "fused_kernel")
+                : launch_process(fused_kernel<TI, TO, 16>, a, n_rows, threads,
+                                 Table<16, false>::bytes(a.slots, bias, len), false, s, "fused_kernel");
+  }
+  const bool stream = !a.in_place || a.r.mask;
+  if (stream) {
+    a.vps = (int)std::min<int64_t>(nv, 2 * kProcAhead * kProcThreads);
+    a.split = (int)((nv + a.vps - 1) / a.vps);
+    if (int st = launch_process(stream_kernel<TI, TO>, a, n_rows * a.split, per_thread(a.vps, kProcAhead, kProcThreads), 0,
+                                false, s, "stream_kernel"))
+      return st;
+  }
+  if (!count) return CNNUE_OK;
+  const int64_t named = len + a.r.bias_count;
+  if (len <= kHashTokens && named <= 2 * kHashTokens) {
+    a.lg = 0;
+    a.slots = 64;
+    while (a.slots < 2 * named) a.slots *= 2;
+    const int threads = len <= 128 * kTokensAhead ? 128 : len <= 256 * kTokensAhead ? 256 : kCountThreads;
+    return launch_process(penalise_kernel<TI, TO, 16, true>, a, n_rows, threads, Table<16, true>::bytes(a.slots, bias, len),
+                          stream, s, "penalise_kernel");
+  }
+  const int64_t most = wide ? 16384 : 32768;  // 64 KB of counters
+  a.lg = 0;
+  while (((int64_t)a.vocab + (1 << a.lg) - 1) >> a.lg > most) ++a.lg;
+  a.slots = (int)(((int64_t)a.vocab + (1 << a.lg) - 1) >> a.lg);
+  return wide ? launch_process(penalise_kernel<TI, TO, 32, false>, a, n_rows << a.lg, kCountThreads,
+                               Table<32, false>::bytes(a.slots, bias, len), stream, s, "penalise_kernel")
+              : launch_process(penalise_kernel<TI, TO, 16, false>, a, n_rows << a.lg, kCountThreads,
+                               Table<16, false>::bytes(a.slots, bias, len), stream, s, "penalise_kernel");
 }
 
 // ---------------------------------------------------------------------------
@@ -1110,7 +1210,7 @@ int cnnue_logits_process(const void* d_logits, int64_t logits_stride, int logits
   if (r.bias_count < 0 || r.bias_count > 0x7fffffff || r.bias_tokens_stride < 0 || r.bias_values_stride < 0)
     return set_error(CNNUE_ERR_INVALID_ARG, "bias: count or stride");
   if (int st = check_mask(r.mask, r.mask_stride, r.mask_rows, r.mask_index, n_rows, vocab)) return st;
-  ProcArgs a{d_logits, d_out, logits_stride, out_stride, (int)vocab, 0, 0, in_place, r, d_status};
+  ProcArgs a{d_logits, d_out, logits_stride, out_stride, (int)vocab, 0, 0, 0, 0, in_place, r, d_status};
   cudaStream_t s = (cudaStream_t)stream;
   if (logits_type == CNNUE_F32) return pick_process<float, float>(a, n_rows, s);
   if (logits_type == CNNUE_BF16)

@@ -113,7 +113,7 @@ def test_process_strides_in_place_and_neighbours(pad, offset, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("vocab", [100, 2086, 20_001])
+@pytest.mark.parametrize("vocab", [100, 2086, 16_384, 16_385, 40_001])
 def test_process_in_place_with_penalties_biases_and_masks_rounds_once(vocab, dtype):
     """The same bits as out of place: biased tokens among the penalised ones, repeated, masked."""
     g = gen(vocab)
@@ -220,6 +220,31 @@ def test_process_bad_data_is_reported_and_skipped():
     assert int(status) == 1 and (out[1] == -math.inf).all() and (out[[0, 2]] == 1).all()
 
 
+@pytest.mark.parametrize("count", [1, 500, 1500, 4000])
+def test_process_long_bias_lists(count):
+    """More entries than threads; more than a hash table holds; every token of the vocabulary named."""
+    R, V = 2, 20_000
+    g = gen(count)
+    x = rows(R, V, torch.float32, g)
+    tok = torch.stack([torch.randperm(V, generator=g)[:count] for _ in range(R)]).int()
+    tok[0, count // 2:] = tok[0, 0]  # one token again and again
+    kw = dict(bias_tokens=tok, bias_values=torch.randn(R, count, generator=g), history=tok.flip(1)[:, :1000],
+              frequency=torch.ones(R), mask=mask_of(1, V, 0.7, g)[0])
+    want, bound = ref.process(x, **kw)
+    ref.close(lg.process_logits(dev(x), **{k: dev(t) for k, t in kw.items()}), want, bound)
+
+
+def test_process_hash_neighbours_and_the_last_token():
+    """Tokens that meet in a hash table, and the ends of a large vocabulary."""
+    V, n = 1 << 20, 1000
+    x = torch.ones(1, V)
+    h = (torch.arange(n) * 1021 % V).int()
+    h[-3:] = torch.tensor([V - 1, 0, V - 1])
+    kw = dict(history=h, frequency=torch.ones(1))
+    want, bound = ref.process(x, **kw)
+    ref.close(lg.process_logits(dev(x), history=dev(h), frequency=dev(torch.ones(1))), want, bound)
+
+
 def test_process_empty():
     assert lg.process_logits(torch.empty(0, 5, device=DEV)).shape == (0, 5)
     x = torch.ones(2, 9, device=DEV)
@@ -229,14 +254,14 @@ def test_process_empty():
     assert torch.equal(out, x)
 
 
-@pytest.mark.parametrize("L", [20_000, 32_767, 32_768, 60_000])
+@pytest.mark.parametrize("L", [1, 2047, 2048, 2049, 5000, 20_000, 32_767, 32_768, 60_000])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_process_long_history_and_large_vocabulary(dtype, L):
     R, V = 3, 100_003
     g = gen(9)
     x = rows(R, V, dtype, g)
     kw = dict(history=history_of(R, V, L, g), frequency=torch.rand(R, generator=g), repetition=1 + torch.rand(R, generator=g),
-              prompt_lengths=torch.tensor([0, 10_000, L], dtype=torch.int32),
+              prompt_lengths=torch.tensor([0, L // 2, L], dtype=torch.int32),
               bias_tokens=torch.randint(0, V, (R, 300), generator=g).int(), bias_values=torch.randn(R, 300, generator=g),
               mask=mask_of(R, V, 0.9, g))
     want, bound = ref.process(x, **kw)
