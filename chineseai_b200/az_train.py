@@ -361,13 +361,20 @@ class AzTrainer:
     AdamW run after the step, from the host.  Either way the step's
     statistics (TrainStats) are the whole batch's (sums over every rank's
     share, samples = the global batch), and a kernel status raised on any
-    rank skips AdamW and raises on every rank."""
+    rank skips AdamW and raises on every rank.
+
+    state_bits=8 keeps AdamW's moments in 8 bits (optim.MultiAdamW over the
+    leaves: 2.03 instead of 8 bytes per parameter); the update then runs after
+    the step's gradients instead of beside them, and a batch with a kernel
+    status changes nothing."""
 
     def __init__(self, weights: "az.AzWeights", lr: float = 1e-3, device: int = 0, weight_decay: float = 1e-4,
                  beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8, graph: bool = False, group=None,
-                 guard=None, native: Optional[bool] = None):
+                 guard=None, native: Optional[bool] = None, state_bits: int = 32):
         import torch
         self.torch = torch
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
         if native is None:
             native = weights.hidden in NATIVE_HIDDEN
         if native and weights.hidden not in NATIVE_HIDDEN:
@@ -405,8 +412,16 @@ class AzTrainer:
         # metrics and status bits through the same all-reduce
         self._tail_at = (pos + _ALIGN - 1) // _ALIGN * _ALIGN
         self.grad = torch.zeros(self._tail_at + _TAIL, dtype=torch.float32, device=self.device)
-        self.m = torch.zeros(self.n_params, dtype=torch.float32, device=self.device)
-        self.v = torch.zeros_like(self.m)
+        self.optimizer = self.m = self.v = None
+        if state_bits == 8:
+            from .optim import MultiAdamW
+            leaves = [slice(off, min(off + n, self.n_params)) for *_, off, n in layout]
+            self.optimizer = MultiAdamW([self.flat[leaf] for leaf in leaves], [self.grad[leaf] for leaf in leaves], lr=lr,
+                                        beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay, state_bits=8,
+                                        device_state=True)
+        else:
+            self.m = torch.zeros(self.n_params, dtype=torch.float32, device=self.device)
+            self.v = torch.zeros_like(self.m)
         self._layout = layout
         self.params = {}
         for name, first, last, shape, off, n in layout:
@@ -447,6 +462,8 @@ class AzTrainer:
     def set_learning_rate(self, lr: float) -> None:
         """GpuTrainer::set_learning_rate (src/az/train_gpu_candle.rs:134-136)."""
         self.lr = lr
+        if self.optimizer is not None:
+            self.optimizer.set_learning_rate(lr)
         self.adam_state[:8].copy_(self.torch.from_numpy(np.array([lr], np.float64).view(np.uint8)))
 
     # -- data ---------------------------------------------------------------
@@ -617,11 +634,19 @@ class AzTrainer:
             out = self.grad[self._tail_at: self._tail_at + _NATIVE_OUT]
             self.native_loss(bt, value_weight, policy_weight, out)
             dist.all_reduce(self.grad, op=dist.ReduceOp.SUM, group=self.group)
+            if self.optimizer is not None:
+                self.optimizer.step(1.0 / self.world, skip=out[_N_METRICS:_N_METRICS + 4])
+                return out
             check(lib().cnnue_adamw_device_scaled(self.flat.data_ptr(), self.m.data_ptr(), self.v.data_ptr(),
                                                   self.grad.data_ptr(), self.n_params, self.adam_state.data_ptr(),
                                                   1.0 / self.world, out[_N_METRICS:].data_ptr(), 4,
                                                   self.torch.cuda.current_stream(self.device).cuda_stream),
                   "cnnue_adamw_device_scaled")
+            return out
+        if self.native and self.optimizer is not None:
+            out = self.native_loss(bt, value_weight, policy_weight)
+            if self.world == 1:
+                self.optimizer.step(skip=out[_N_METRICS:_N_METRICS + 4])
             return out
         if self.native:
             return self.native_loss(bt, value_weight, policy_weight, adamw=self.world == 1)
@@ -629,11 +654,16 @@ class AzTrainer:
         self.status.zero_()
         loss, metrics = self.loss(self.expand(bt), value_weight, policy_weight)
         loss.backward()
-        if self.world == 1:
+        if self.world == 1 and self.optimizer is not None:
+            self.optimizer.step(skip=self.status.float())
+        elif self.world == 1:
             self._adamw()
         return self.torch.cat([metrics, self.status.float()])
 
     def _adamw(self) -> None:
+        if self.optimizer is not None:
+            self.optimizer.step()
+            return
         check(lib().cnnue_adamw_device(self.flat.data_ptr(), self.m.data_ptr(), self.v.data_ptr(),
                                        self.grad.data_ptr(), self.n_params, self.adam_state.data_ptr(),
                                        self.torch.cuda.current_stream(self.device).cuda_stream),

@@ -134,3 +134,12 @@ class ResNetModel:
                                      logits.data_ptr() if logits is not None else None, value.data_ptr(),
                                      ws.data_ptr(), ws.numel(), s.cuda_stream), "cnnue_rn_forward")
         return probs, logits, value
+
+    def move_logits(self, planes, **rules):
+        """(logits [B][2086], value [B]) with what a caller lets the net answer:
+        `rules` are those of logits.process_logits (mask=..., the packed legal
+        moves of mcts.legal_mask; history and penalties; biases), applied to the
+        logits in place.  A move that is not allowed has logit -inf."""
+        from .logits import process_logits
+        _, logits, value = self.forward(planes, with_logits=True)
+        return process_logits(logits, out=logits, **rules), value

@@ -547,6 +547,8 @@ def test_legal_moves_choose_learn_and_update():
     a = ref.unpack(mask.cpu(), 2086)
     want, bound = ref.process(logits.cpu(), mask=mask.cpu())
     ref.close(lg.process_logits(logits, mask=mask), want, bound)
+    answer, _ = model.move_logits(planes, mask=mask)
+    ref.close(answer, want, bound)
     model.close()
 
     g = gen(1)

@@ -310,3 +310,40 @@ def test_results_do_not_change_from_run_to_run():
             opt.step()
         got.append(torch.cat([t.float() for t in p] + [t.float() for t in opt.state["v"]]))
     assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("native", [True, False])
+def test_az_trainer_with_8_bit_states(native, graph):
+    """The first step from zero moments is the 32-bit trainer's (the update comes before the rounding, and root and
+    quotient are good to 2^-21 of the step); later steps stay near it, replayed or not; a bad batch changes nothing."""
+    from chineseai_b200 import az, az_train
+    from chineseai_b200._lib import CnnueError
+    w = az.AzWeights.random(32, 7)
+    batch = az_train.pack_batch(az_train.random_samples(48, 5), caps=(96, 160, 256), fixed=True)
+    a = az_train.AzTrainer(w, lr=LR, graph=graph, native=native)
+    b = az_train.AzTrainer(w, lr=LR, graph=graph, native=native, state_bits=8)
+    start = a.flat.clone()
+    sa, sb = a.step(batch), b.step(batch)
+    assert sa.loss == sb.loss or not native
+    move = (a.flat - start).abs()
+    # gradients of the autograd path may differ by their summation; the native step's are the same bits
+    if native:
+        assert ((a.flat - b.flat).abs() <= 4 * EPS32 * start.abs() + (2.0 ** -20 + 16 * EPS32) * move + 2.0 ** -140).all()
+    for _ in range(3):
+        sa, sb = a.step(batch), b.step(batch)
+    assert b.optimizer.step_count == 4 and torch.isfinite(b.flat).all()
+    # with nearly constant gradients each of the 3 later steps moves a parameter by about lr, on either side by moments
+    # that are good to 2^-4 each (m over its root)
+    assert (a.flat - b.flat).abs().max() < 3 * LR * (1 + (1 + 2.0 ** -4) / (1 - 2.0 ** -4)) * 1.01
+    before = b.flat.clone()
+    bad = az_train.pack_batch(az_train.random_samples(48, 5), caps=(96, 160, 256), fixed=True)
+    bad.feature_items[3, 0] = 1700
+    with pytest.raises(CnnueError):
+        b.step(bad)
+    assert torch.equal(b.flat, before) and b.optimizer.step_count == 4
+    b.set_learning_rate(0.0)
+    b.step(batch)
+    assert torch.equal(b.flat, before * 1.0) and b.optimizer.step_count == 5
+    a.close()
+    b.close()
