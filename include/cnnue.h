@@ -594,8 +594,8 @@ int cnnue_adamw_device_scaled(float* d_params, float* d_m, float* d_v, const flo
  *   scale = max|x| * (1/448) (0 when that is below 2^-126), code = e4m3(x *
  *   (448 / max|x|)) rounded to nearest even, u' > 0 never below 2^-9 of the
  *   scale (a second moment above zero stays above zero)
- * in fp32, with the square root and the quotient good to 2^-22 and v' below
- * 2^-126 taken as 0; the update uses m' and u' before they are rounded to 8
+ * in fp32 (u' good to 0.501 of its last place, the step's quotient to 2^-22;
+ * a v' below 2^-126 gives a u' below 2^-62); the update uses m' and u' before they are rounded to 8
  * bits.  A NaN or infinity in a block's m' (u') makes the scale and the codes of that
  * block's m (u) non-finite.
  * copy (optional): the updated parameter rounded to copy_type (bf16 or fp16),
