@@ -23,6 +23,7 @@ import numpy as np
 import torch
 
 from ._lib import check, lib
+from .quantized import _device_stream
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -115,14 +116,6 @@ def _mask(mask: Optional[torch.Tensor], mask_index, n: int, vocab: int, dev: int
         _per_row(mask_index, n, dev, torch.int32, "mask_index", keep)
 
 
-def _current_stream(dev: int) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
-
-
-# the same handle without the Stream object around it, where torch has the call
-_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
-
-
 def _call(name: str, dev: int, status: Optional[torch.Tensor], *args) -> None:
     """One entry point on the device's current stream.  With `status` None the
     kernels' status word is read here (a host synchronisation) and raised."""
@@ -134,7 +127,7 @@ def _call(name: str, dev: int, status: Optional[torch.Tensor], *args) -> None:
         status = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", dev))
     elif status.dtype is not torch.int32 or status.get_device() != dev or status.numel() < 1:
         raise ValueError(f"status must be an int32 tensor on cuda:{dev}")
-    stream = _stream(dev)
+    stream = _device_stream(dev)
     handle = lib()
     st = getattr(handle, name)(*args, status.data_ptr(), stream)
     if st:

@@ -7,21 +7,22 @@ parameters and gradients.
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional, Sequence
 
 import numpy as np
 import torch
 
-from ._lib import AdamwTensor, check, lib
+from ._lib import check, lib
+from .quantized import _device_stream
 
 BLOCK = 256     # elements per scale of an 8-bit state
 NO_DECAY = 1    # cnnue_adamw_tensor flag
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _span(t: torch.Tensor):
-    return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+# cnnue_adamw_tensor
+_TENSOR = np.dtype([(k, np.uint64) for k in ("param", "grad", "m", "v", "m_scale", "v_scale", "copy")] + [("n", np.int64)]
+                   + [(k, np.int16) for k in ("param_type", "grad_type", "copy_type", "flags")])
 
 
 class MultiAdamW:
@@ -55,7 +56,7 @@ class MultiAdamW:
                  no_decay: Optional[Sequence[bool]] = None, step: int = 0, device_state: bool = False):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
-        self.params = [p.detach() for p in params]
+        self.params = list(params)
         if not self.params:
             raise ValueError("no parameters")
         self.device = self.params[0].device
@@ -65,44 +66,25 @@ class MultiAdamW:
         self.state_bits = state_bits
         self.lr, self.beta1, self.beta2, self.eps, self.weight_decay = lr, beta1, beta2, eps, weight_decay
         self._step = step
-        for i, p in enumerate(self.params):
-            self._check(p, f"params[{i}]", _TYPES, None)
-        state = state or {}
-        names = ("m", "v") if state_bits == 32 else ("m", "v", "m_scale", "v_scale")
-        if state and set(state) != set(names):
-            raise ValueError(f"state must hold {names}, has {tuple(state)}")
-        self.state = {}
-        for k in names:
-            scale = k.endswith("_scale")
-            dtype = torch.float8_e4m3fn if state_bits == 8 and not scale else torch.float32
-            size = [(p.numel() + BLOCK - 1) // BLOCK if scale else p.numel() for p in self.params]
-            if state:
-                if len(state[k]) != n:
-                    raise ValueError(f"state {k} has {len(state[k])} tensors for {n} parameters")
-                for i, t in enumerate(state[k]):
-                    self._check(t, f"state {k}[{i}]", (dtype,), size[i])
-                self.state[k] = list(state[k])
-            else:  # one buffer, every tensor on a 256-byte boundary
-                each = torch.empty(0, dtype=dtype).element_size()
-                places = np.concatenate([[0], np.cumsum([(s * each + 255) // 256 * 256 for s in size])])
-                flat = torch.zeros(int(places[-1]), dtype=torch.uint8, device=self.device)
-                self.state[k] = [flat[a:a + s * each].view(dtype) for a, s in zip(places.tolist(), size)]
+        self._table = np.zeros(n, _TENSOR)
+        self._address = self._table.ctypes.data
+        self._sizes = [p.numel() for p in self.params]
+        self._table["n"] = self._sizes
+        self._table["param_type"] = self._buffers("params", self.params, _TYPES, self._sizes, "param")
+        self._hold_state(state or {})
         copies = [None] * n if copies is None else list(copies)
         if len(copies) != n or (no_decay is not None and len(no_decay) != n):
             raise ValueError("copies and no_decay have one entry per parameter")
-        for i, c in enumerate(copies):
-            if c is not None:
-                self._check(c, f"copies[{i}]", (torch.bfloat16, torch.float16), self.params[i].numel())
         self.copies = copies
-        self._table = (AdamwTensor * n)()
-        for i, (e, p) in enumerate(zip(self._table, self.params)):
-            e.param, e.n, e.param_type = p.data_ptr(), p.numel(), _TYPES[p.dtype]
-            e.m, e.v = self.state["m"][i].data_ptr(), self.state["v"][i].data_ptr()
-            if state_bits == 8:
-                e.m_scale, e.v_scale = self.state["m_scale"][i].data_ptr(), self.state["v_scale"][i].data_ptr()
-            if copies[i] is not None:
-                e.copy, e.copy_type = copies[i].data_ptr(), _TYPES[copies[i].dtype]
-            e.flags = NO_DECAY if no_decay is not None and no_decay[i] else 0
+        with_copy = [i for i, c in enumerate(copies) if c is not None]
+        if with_copy:
+            some = [copies[i] for i in with_copy]
+            types = self._buffers("copies", some, (torch.bfloat16, torch.float16), [self._sizes[i] for i in with_copy])
+            self._table["copy"][with_copy] = [c.data_ptr() for c in some]
+            self._table["copy_type"][with_copy] = types
+        if no_decay is not None:
+            self._table["flags"] = [NO_DECAY if d else 0 for d in no_decay]
+        self._check_written()
         self._dstate = None
         if device_state:
             host = np.zeros(12, np.float64)
@@ -111,39 +93,80 @@ class MultiAdamW:
             self._dstate = torch.from_numpy(host.view(np.uint8).copy()).to(self.device)
         self.bind(grads)
 
-    def _check(self, t: torch.Tensor, name: str, dtypes, size: Optional[int]) -> None:
-        if t.device != self.device:
-            raise ValueError(f"{name} must be on {self.device}, is on {t.device}")
-        if t.dtype not in dtypes:
-            raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-        if size is not None and t.numel() != size:
-            raise ValueError(f"{name} must hold {size} elements, has {t.numel()}")
+    def _buffers(self, name: str, tensors, dtypes, sizes, column: Optional[str] = None) -> list:
+        """Checks the buffers, writes their addresses to a column of the
+        table; returns their type codes (None for state types)."""
+        dev = self.device.index
+        for i, (t, size) in enumerate(zip(tensors, sizes)):
+            if t.dtype not in dtypes:
+                raise TypeError(f"{name}[{i}] must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+            if t.get_device() != dev:
+                raise ValueError(f"{name}[{i}] must be on {self.device}, is on {t.device}")
+            if not t.is_contiguous():
+                raise ValueError(f"{name}[{i}] must be contiguous")
+            if t.numel() != size:
+                raise ValueError(f"{name}[{i}] must hold {size} elements, has {t.numel()}")
+        if column is not None:
+            self._table[column] = [t.data_ptr() for t in tensors]
+        return [_TYPES.get(t.dtype) for t in tensors]
+
+    def _hold_state(self, state: dict) -> None:
+        eight = self.state_bits == 8
+        names = ("m", "v", "m_scale", "v_scale") if eight else ("m", "v")
+        if state and set(state) != set(names):
+            raise ValueError(f"state must hold {names}, has {tuple(state)}")
+        self.state = {}
+        for k in names:
+            scale = k.endswith("_scale")
+            dtype = torch.float8_e4m3fn if eight and not scale else torch.float32
+            sizes = [-(-s // BLOCK) for s in self._sizes] if scale else self._sizes
+            if state:
+                if len(state[k]) != len(sizes):
+                    raise ValueError(f"state {k} has {len(state[k])} tensors for {len(sizes)} parameters")
+                self.state[k] = list(state[k])
+            else:  # one buffer, every tensor on a 256-byte boundary
+                each = 1 if dtype is torch.float8_e4m3fn else 4
+                places = np.concatenate([[0], np.cumsum([(s * each + 255) // 256 * 256 for s in sizes])]).tolist()
+                flat = torch.zeros(places[-1], dtype=torch.uint8, device=self.device)
+                self.state[k] = [flat[a:a + s * each].view(dtype) for a, s in zip(places, sizes)]
+            self._buffers(f"state {k}", self.state[k], (dtype,), sizes, k)
+
+    def _check_written(self) -> None:
+        """No buffer that is written shares memory with another one."""
+        t, n = self._table, self._table["n"]
+        blocks = -(-n // BLOCK)
+        each = 1 if self.state_bits == 8 else 4
+        spans = [(t["param"], n * np.where(t["param_type"] == 0, 4, 2), "params"), (t["m"], n * each, "state m"),
+                 (t["v"], n * each, "state v"), (t["copy"], np.where(t["copy"] != 0, n * 2, 0), "copies")]
+        if self.state_bits == 8:
+            spans += [(t["m_scale"], blocks * 4, "state m_scale"), (t["v_scale"], blocks * 4, "state v_scale")]
+        lo = np.concatenate([s[0] for s in spans]).astype(np.int64)
+        size = np.concatenate([s[1] for s in spans])
+        kind = np.repeat([s[2] for s in spans], len(n))
+        order = np.argsort(lo, kind="stable")
+        order = order[size[order] > 0]
+        lo, hi, kind = lo[order], (lo + size)[order], kind[order]
+        clash = np.nonzero(lo[1:] < np.maximum.accumulate(hi)[:-1])[0]
+        if len(clash):
+            raise ValueError(f"{kind[clash[0] + 1]} overlaps {kind[clash[0]]}")
+        self._written = lo, hi, kind
 
     def bind(self, grads: Sequence[torch.Tensor]) -> None:
         """The gradient buffers that the following steps read."""
         grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
-        for i, (g, p) in enumerate(zip(grads, self.params)):
-            self._check(g, f"grads[{i}]", _TYPES, p.numel())
-        # a buffer that is written may not share memory with any other
-        spans = [(*_span(t), True, k) for k, ts in (("params", self.params), *self.state.items(), ("copies", self.copies))
-                 for t in ts if t is not None and t.numel()]
-        spans += [(*_span(g), False, "grads") for g in grads if g.numel()]
-        spans.sort(key=lambda s: (s[0], s[1]))
-        end, end_written, kind, last = 0, 0, "", ""
-        for lo, hi, written, k in spans:
-            if lo < end_written or (written and lo < end):
-                raise ValueError(f"{k} overlaps {last if lo < end_written else kind}")
-            if hi > end:
-                end, kind = hi, k
-            if written and hi > end_written:
-                end_written, last = hi, k
+        types = np.array(self._buffers("grads", grads, _TYPES, self._sizes))
+        g_lo = np.array([g.data_ptr() for g in grads], np.int64)
+        g_hi = g_lo + self._table["n"] * np.where(types == 0, 4, 2)
+        lo, hi, kind = self._written
+        if len(lo):
+            before = np.searchsorted(lo, g_hi, "left") - 1  # the last written buffer that starts before the gradient ends
+            clash = np.nonzero((before >= 0) & (hi[before] > g_lo) & (g_hi > g_lo))[0]
+            if len(clash):
+                raise ValueError(f"grads[{clash[0]}] overlaps {kind[before[clash[0]]]}")
         self.grads = grads
-        for e, g in zip(self._table, grads):
-            e.grad, e.grad_type = g.data_ptr(), _TYPES[g.dtype]
+        self._table["grad"], self._table["grad_type"] = g_lo, types
 
     @property
     def step_count(self) -> int:
@@ -170,14 +193,14 @@ class MultiAdamW:
         return self._run(grad_scale, skip)
 
     def _run(self, grad_scale: float, skip: Optional[torch.Tensor]) -> None:
-        stream = torch.cuda.current_stream(self.device).cuda_stream
+        stream = _device_stream(self.device.index)
         flags = (None, 0) if skip is None else (skip.data_ptr(), skip.numel())
         if self._dstate is not None:
-            check(lib().cnnue_adamw_multi_device(C.addressof(self._table), len(self._table), self.state_bits,
+            check(lib().cnnue_adamw_multi_device(self._address, len(self.params), self.state_bits,
                                                  self._dstate.data_ptr(), grad_scale, *flags, stream),
                   "cnnue_adamw_multi_device")
             return
-        check(lib().cnnue_adamw_multi(C.addressof(self._table), len(self._table), self.state_bits, self.lr, self.beta1,
+        check(lib().cnnue_adamw_multi(self._address, len(self.params), self.state_bits, self.lr, self.beta1,
                                       self.beta2, self.eps, self.weight_decay, self._step + 1, grad_scale, *flags,
                                       stream), "cnnue_adamw_multi")
         self._step += 1

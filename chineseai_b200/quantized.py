@@ -25,6 +25,15 @@ def _stream_ptr(stream: Optional[torch.cuda.Stream]) -> int:
     return s.cuda_stream
 
 
+def _device_stream(index: int) -> int:
+    """The handle of a device's current stream."""
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same without the Stream object around it, where torch has the call
+_device_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _device_stream)
+
+
 def as_device(a: np.ndarray, device: torch.device) -> torch.Tensor:
     """Copies a numpy array to the device as raw bytes of the same width
     (uint16 -> int16, uint32 -> int32 views; only the pointer matters)."""

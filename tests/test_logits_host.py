@@ -74,6 +74,14 @@ def test_packed_structs_have_the_declared_layout(packed, declared):
     assert [getattr(back, name) for name, _ in declared._fields_] == values
 
 
+def test_optimizer_table_has_the_declared_layout():
+    from chineseai_b200.optim import _TENSOR
+    assert _TENSOR.itemsize == C.sizeof(_lib.AdamwTensor)
+    for name, kind in _lib.AdamwTensor._fields_:
+        assert _TENSOR.fields[name][1] == getattr(_lib.AdamwTensor, name).offset
+        assert _TENSOR.fields[name][0].itemsize == C.sizeof(kind)
+
+
 A, B, S = 1 << 20, 1 << 24, 1 << 28  # addresses that no call below gets to use
 
 
