@@ -1135,10 +1135,9 @@ int check_rows(const void* p, int64_t stride, int type, int64_t n_rows, int64_t 
   return CNNUE_OK;
 }
 
-int check_mask(const uint32_t* mask, int64_t stride, int64_t mask_rows, const int32_t* index, int64_t n_rows, int64_t vocab) {
+int check_mask(const uint32_t* mask, int64_t stride, int64_t mask_rows, const int32_t* index, int64_t n_rows) {
   if (!mask) return index ? set_error(CNNUE_ERR_INVALID_ARG, "mask_index without a mask") : CNNUE_OK;
-  if (mask_rows < 0 || stride < 0 || (mask_rows > 1 && stride < (vocab + 31) / 32))
-    return set_error(CNNUE_ERR_INVALID_ARG, "mask: rows or stride");
+  if (mask_rows < 0 || stride < 0) return set_error(CNNUE_ERR_INVALID_ARG, "mask: rows or stride");
   if (!index && mask_rows != 1 && mask_rows != n_rows)
     return set_error(CNNUE_ERR_INVALID_ARG, "mask: %lld rows for %lld rows of logits", (long long)mask_rows,
                      (long long)n_rows);
@@ -1165,7 +1164,20 @@ int check_targets(const cnnue_loss_targets* t, int64_t n_rows, int64_t vocab) {
     if (t->count < 0 || t->index_stride < 0 || t->prob_stride < 0)
       return set_error(CNNUE_ERR_INVALID_ARG, "targets: negative size");
   }
-  return check_mask(t->mask, t->mask_stride, t->mask_rows, t->mask_index, n_rows, vocab);
+  return check_mask(t->mask, t->mask_stride, t->mask_rows, t->mask_index, n_rows);
+}
+
+// The gradient may share memory with neither the logits nor dense targets:
+// both are read again after parts of it are written.
+int check_grad(const void* grad, int64_t grad_stride, const void* z, int64_t z_stride, int type, const cnnue_loss_targets* t,
+               int64_t n_rows, int64_t vocab) {
+  if (int st = check_rows(grad, grad_stride, type, n_rows, vocab, true, "grad")) return st;
+  const int b = element_bytes(type);
+  if (overlap(z, z_stride, b, grad, grad_stride, b, n_rows, vocab))
+    return set_error(CNNUE_ERR_INVALID_ARG, "grad overlaps the logits");
+  if (t->dense && overlap(t->dense, t->dense_stride, element_bytes(t->dense_type), grad, grad_stride, b, n_rows, vocab))
+    return set_error(CNNUE_ERR_INVALID_ARG, "grad overlaps the targets");
+  return CNNUE_OK;
 }
 
 int check_shape(int64_t n_rows, int64_t vocab, const uint32_t* status) {
@@ -1209,7 +1221,7 @@ int cnnue_logits_process(const void* d_logits, int64_t logits_stride, int logits
     return set_error(CNNUE_ERR_INVALID_ARG, "bias tokens and values come together");
   if (r.bias_count < 0 || r.bias_count > 0x7fffffff || r.bias_tokens_stride < 0 || r.bias_values_stride < 0)
     return set_error(CNNUE_ERR_INVALID_ARG, "bias: count or stride");
-  if (int st = check_mask(r.mask, r.mask_stride, r.mask_rows, r.mask_index, n_rows, vocab)) return st;
+  if (int st = check_mask(r.mask, r.mask_stride, r.mask_rows, r.mask_index, n_rows)) return st;
   ProcArgs a{d_logits, d_out, logits_stride, out_stride, (int)vocab, 0, 0, 0, 0, in_place, r, d_status};
   cudaStream_t s = (cudaStream_t)stream;
   if (logits_type == CNNUE_F32) return pick_process<float, float>(a, n_rows, s);
@@ -1240,11 +1252,8 @@ int cnnue_policy_loss_bwd(const void* d_logits, int64_t logits_stride, int logit
   if (int st = check_targets(targets, n_rows, vocab)) return st;
   if (vocab == 0) return set_error(CNNUE_ERR_INVALID_ARG, "empty vocabulary");
   if (int st = check_rows(d_logits, logits_stride, logits_type, n_rows, vocab, false, "logits")) return st;
-  if (int st = check_rows(d_grad, grad_stride, logits_type, n_rows, vocab, true, "grad")) return st;
+  if (int st = check_grad(d_grad, grad_stride, d_logits, logits_stride, logits_type, targets, n_rows, vocab)) return st;
   if (!d_stats) return set_error(CNNUE_ERR_INVALID_ARG, "null stats");
-  const int b = element_bytes(logits_type);
-  if (overlap(d_logits, logits_stride, b, d_grad, grad_stride, b, n_rows, vocab))
-    return set_error(CNNUE_ERR_INVALID_ARG, "grad overlaps the logits");
   const LossArgs a{d_logits,   logits_stride, (int)vocab, 0, 0, n_rows, *targets, d_upstream, nullptr, const_cast<float*>(d_stats),
                    d_grad, grad_stride, d_status};
   return pick_loss<false, true>(a, logits_type, n_rows, (cudaStream_t)stream);
@@ -1258,11 +1267,8 @@ int cnnue_policy_loss_grad(const void* d_logits, int64_t logits_stride, int logi
   if (int st = check_targets(targets, n_rows, vocab)) return st;
   if (vocab == 0) return set_error(CNNUE_ERR_INVALID_ARG, "empty vocabulary");
   if (int st = check_rows(d_logits, logits_stride, logits_type, n_rows, vocab, false, "logits")) return st;
-  if (int st = check_rows(d_grad, grad_stride, logits_type, n_rows, vocab, true, "grad")) return st;
+  if (int st = check_grad(d_grad, grad_stride, d_logits, logits_stride, logits_type, targets, n_rows, vocab)) return st;
   if (!d_loss) return set_error(CNNUE_ERR_INVALID_ARG, "null loss");
-  const int b = element_bytes(logits_type);
-  if (overlap(d_logits, logits_stride, b, d_grad, grad_stride, b, n_rows, vocab))
-    return set_error(CNNUE_ERR_INVALID_ARG, "grad overlaps the logits");
   const LossArgs a{d_logits, logits_stride, (int)vocab, 0, 0, n_rows, *targets, nullptr, d_loss, nullptr, d_grad, grad_stride, d_status};
   return pick_loss<true, true>(a, logits_type, n_rows, (cudaStream_t)stream);
 }

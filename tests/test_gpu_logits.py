@@ -138,6 +138,8 @@ def test_process_broadcast_row_and_transposed_logits():
     m = mask_of(4, 500, 0.5, g)
     want, bound = ref.process(x.expand(4, -1), mask=m)
     ref.close(lg.process_logits(dev(x).expand(4, -1), mask=dev(m)), want, bound)
+    want, bound = ref.process(x.expand(4, -1), mask=m[:1].expand(4, -1))
+    ref.close(lg.process_logits(dev(x).expand(4, -1), mask=dev(m)[:1].expand(4, -1)), want, bound)
     t = torch.randn(500, 4, generator=g)
     want, bound = ref.process(t.t(), mask=m)
     ref.close(lg.process_logits(dev(t).t(), mask=dev(m)), want, bound)
@@ -268,25 +270,57 @@ def test_process_long_history_and_large_vocabulary(dtype, L):
     ref.close(lg.process_logits(dev(x), **{k: dev(t) for k, t in kw.items()}), want, bound, dtype)
 
 
-def test_process_captured_and_replayed_on_new_data():
+@pytest.mark.parametrize("V,L", [(2086, 64), (40_000, 64), (40_000, 4000)])
+def test_process_captured_and_replayed_on_new_data(V, L):
+    """One launch, and two that overlap (short and long histories); two graphs of the same buffers in turn."""
     g = gen(3)
-    R, V = 4, 2086
-    x, h, n = dev(rows(R, V, torch.float32, g)), dev(history_of(R, V, 64, g)), dev(torch.full((R,), 10, dtype=torch.int32))
-    f = dev(torch.rand(R, generator=g))
+    R = 4
+    x, h, n = dev(rows(R, V, torch.float32, g)), dev(history_of(R, V, L, g)), dev(torch.full((R,), 10, dtype=torch.int32))
+    f, m = dev(torch.rand(R, generator=g)), dev(mask_of(R, V, 0.5, g))
     status = torch.zeros(1, dtype=torch.int32, device=DEV)
     out = torch.empty_like(x)
-    lg.process_logits(x, history=h, lengths=n, frequency=f, out=out, status=status)
+    kw = dict(history=h, lengths=n, frequency=f, mask=m)
+    lg.process_logits(x, out=out, status=status, **kw)
     torch.cuda.synchronize()
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        lg.process_logits(x, history=h, lengths=n, frequency=f, out=out, status=status)
-    for k in (20, 64):
-        n.fill_(k)
-        x.mul_(0.5)
-        graph.replay()
-        want, bound = ref.process(x.cpu(), history=h.cpu(), lengths=n.cpu(), frequency=f.cpu())
-        ref.close(out, want, bound)
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            lg.process_logits(x, out=out, status=status, **kw)
+    for k in (20, L):
+        for graph in graphs:
+            n.fill_(k)
+            x.mul_(0.5)
+            graph.replay()
+            want, bound = ref.process(x.cpu(), **{k: t.cpu() for k, t in kw.items()})
+            ref.close(out, want, bound)
     assert int(status) == 0
+
+
+def test_process_calls_in_a_row_and_on_two_streams():
+    """Calls that follow each other without a wait, the output of one the input of the next, and two streams at once."""
+    g = gen(21)
+    R, V = 8, 30_000
+    x = rows(R, V, torch.bfloat16, g)
+    h = history_of(R, V, 300, g)
+    kw = dict(history=h, frequency=torch.rand(R, generator=g), mask=mask_of(R, V, 0.5, g))
+    d = {k: dev(t) for k, t in kw.items()}
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    first = lg.process_logits(dev(x), **d).cpu()
+    second = lg.process_logits(first.to(DEV), **d).cpu()
+    third = lg.process_logits(second.to(DEV), **d).cpu()
+    a = dev(x)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                y = lg.process_logits(a, status=status, **d)
+                y = lg.process_logits(y, status=status, **d)
+                lg.process_logits(y, out=y, status=status, **d)
+                got.append(y)
+    torch.cuda.synchronize()
+    assert all(torch.equal(y.cpu(), third) for y in got) and int(status) == 0
 
 
 def test_process_on_another_stream():
@@ -491,6 +525,28 @@ def test_loss_bad_tokens_are_reported_and_skipped():
     want, g, bl, bg = ref.loss(x, target_index=torch.tensor([[3, -1], [-1, 4]]))
     ref.close(loss, want, bl)
     ref.close(grad, g, bg)
+
+
+def test_loss_gradient_may_not_replace_its_inputs():
+    x, t = torch.randn(2, 64, device=DEV), torch.rand(2, 64, device=DEV)
+    for grad in (x, t):
+        with pytest.raises(CnnueError, match="overlaps"):
+            lg.policy_loss_grad(x, t, grad=grad)
+
+
+def test_loss_survives_offloaded_and_released_tensors():
+    """Saved-tensor hooks bring other storage to the backward pass; a second pass over a kept graph gives the same."""
+    g = gen(22)
+    x, kw = loss_inputs(3, 700, torch.float32, "lists", g)
+    d = {k: dev(t) for k, t in kw.items()}
+    leaf = dev(x).requires_grad_(True)
+    plain = torch.autograd.grad(lg.policy_loss(leaf, **d).sum(), leaf)[0]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(DEV)):
+        loss = lg.policy_loss(leaf, **d)
+    assert torch.equal(torch.autograd.grad(loss.sum(), leaf)[0], plain)
+    loss = lg.policy_loss(leaf.t().contiguous().t(), **d)  # a copy is made of it
+    first = torch.autograd.grad(loss.sum(), leaf, retain_graph=True)[0]
+    assert torch.equal(first, plain) and torch.equal(torch.autograd.grad(loss.sum(), leaf)[0], plain)
 
 
 def test_loss_empty():

@@ -98,7 +98,7 @@ def process(r=None, logits=A, ls=100, lt=0, out=B, os=100, ot=0, rows=4, vocab=1
     dict(r=dict(history=A, history_bytes=4, history_len=-1)), dict(r=dict(history=A, history_bytes=4, history_len=1 << 31)),
     dict(r=dict(history=A, history_bytes=8, history_stride=-1)), dict(r=dict(bias_tokens=A)), dict(r=dict(bias_values=A)),
     dict(r=dict(bias_tokens=A, bias_values=A, bias_count=-1)), dict(r=dict(mask_index=A)),
-    dict(r=dict(mask=A, mask_rows=3, mask_stride=4)), dict(r=dict(mask=A, mask_rows=4, mask_stride=3)),
+    dict(r=dict(mask=A, mask_rows=3, mask_stride=4)), dict(r=dict(mask=A, mask_rows=4, mask_stride=-1)),
     dict(r=dict(mask=A, mask_rows=-1, mask_stride=4, mask_index=A)),
 ])
 def test_process_refuses(bad):
@@ -126,7 +126,7 @@ def targets(**kw):
     dict(loss=None), dict(lt=4), dict(logits=A + 1), dict(grad=A), dict(grad=A + 4), dict(gs=99), dict(ls=-5),
     dict(t=dict(index=None)), dict(t=dict(dense=A)), dict(t=dict(index_bytes=2)), dict(t=dict(count=-1)),
     dict(t=dict(index_stride=-1)), dict(t=dict(index=None, dense=A, dense_type=7)),
-    dict(t=dict(index=None, dense=A + 2)), dict(t=dict(index=None, dense=A, prob=A)),
+    dict(t=dict(index=None, dense=A + 2)), dict(t=dict(index=None, dense=B, dense_stride=100)), dict(t=dict(index=None, dense=A, prob=A)),
     dict(t=dict(mask=A, mask_rows=2, mask_stride=4)), dict(t=dict(mask_index=A)),
 ])
 def test_loss_refuses(bad):
@@ -136,7 +136,7 @@ def test_loss_refuses(bad):
     L = _lib.lib()
     head = (kw["logits"], kw["ls"], kw["lt"], kw["rows"], kw["vocab"], C.addressof(t))
     assert L.cnnue_policy_loss_grad(*head, kw["loss"], kw["grad"], kw["gs"], kw["status"], None) == INVALID
-    if kw["loss"] is not None and not {"grad", "gs"} & set(bad):
+    if kw["loss"] is not None and not {"grad", "gs"} & set(bad) and kw["t"].get("dense") != B:
         assert L.cnnue_policy_loss_fwd(*head, A, A, kw["status"], None) == INVALID
     if kw["loss"] is not None:
         assert L.cnnue_policy_loss_bwd(*head, A, None, kw["grad"], kw["gs"], kw["status"], None) == INVALID
