@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kProcThreads, 8) stream_kernel(const __grid_co
 }
 
 template <typename TI, typename TO, int BITS>
-__global__ void __launch_bounds__(kProcThreads, 4) fused_kernel(const __grid_constant__ ProcArgs a) {
+__global__ void __launch_bounds__(kProcThreads, 5) fused_kernel(const __grid_constant__ ProcArgs a) {
   extern __shared__ uint4 smem[];
   const int64_t row = blockIdx.x;
   const TI* in = (const TI*)a.in + row * a.in_stride;

@@ -64,16 +64,16 @@ def _per_row(x: Optional[torch.Tensor], n: int, dev: int, dtype: torch.dtype, na
     """Address of a per-row vector, 0 for None."""
     if x is None:
         return 0
+    if x.dtype is dtype and x.get_device() == dev and x.dim() == 1 and x.numel() == n:
+        if not x.is_contiguous():
+            x = x.contiguous()
+            keep.append(x)
+        return x.data_ptr()
     if x.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {x.dtype}")
     if x.get_device() != dev:
         raise ValueError(f"{name} must be on cuda:{dev}, is on {x.device}")
-    if x.dim() != 1 or x.size(0) != n:
-        raise ValueError(f"{name} must be [{n}], got {tuple(x.shape)}")
-    if not x.is_contiguous():
-        x = x.contiguous()
-        keep.append(x)
-    return x.data_ptr()
+    raise ValueError(f"{name} must be [{n}], got {tuple(x.shape)}")
 
 
 def _lists(x: torch.Tensor, n: int, dev: int, dtypes, name: str, keep: list) -> Tuple[int, int, int]:
@@ -82,15 +82,18 @@ def _lists(x: torch.Tensor, n: int, dev: int, dtypes, name: str, keep: list) -> 
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {x.dtype}")
     if x.get_device() != dev:
         raise ValueError(f"{name} must be on cuda:{dev}, is on {x.device}")
-    dim = x.dim()
-    if dim not in (1, 2) or (dim == 2 and x.size(0) != n):
-        raise ValueError(f"{name} must be [{n}, n] or [n], got {tuple(x.shape)}")
-    length = x.size(-1)
-    if length > 1 and x.stride(-1) != 1:
+    shape = x.shape
+    dim = len(shape)
+    if dim not in (1, 2) or (dim == 2 and shape[0] != n):
+        raise ValueError(f"{name} must be [{n}, n] or [n], got {tuple(shape)}")
+    length = shape[-1]
+    strides = x.stride()
+    if length > 1 and strides[-1] != 1:
         x = x.contiguous()
         keep.append(x)
+        strides = x.stride()
     # an empty list has no storage and is never read: any address says that it is there
-    return x.data_ptr() or 1 << 12, (x.stride(0) if dim == 2 else 0), length
+    return x.data_ptr() or 1 << 12, (strides[0] if dim == 2 else 0), length
 
 
 def _mask(mask: Optional[torch.Tensor], mask_index, n: int, vocab: int, dev: int, keep: list):
@@ -103,17 +106,20 @@ def _mask(mask: Optional[torch.Tensor], mask_index, n: int, vocab: int, dev: int
         raise TypeError(f"mask must hold packed int32 words (pack_mask), got {mask.dtype}")
     if mask.get_device() != dev:
         raise ValueError(f"mask must be on cuda:{dev}, is on {mask.device}")
-    words, dim = (vocab + 31) // 32, mask.dim()
-    if dim not in (1, 2) or mask.size(-1) != words:
-        raise ValueError(f"mask must be [masks, {words}] or [{words}], got {tuple(mask.shape)}")
-    if words > 1 and mask.stride(-1) != 1:
+    words, shape = (vocab + 31) // 32, mask.shape
+    dim = len(shape)
+    if dim not in (1, 2) or shape[-1] != words:
+        raise ValueError(f"mask must be [masks, {words}] or [{words}], got {tuple(shape)}")
+    strides = mask.stride()
+    if words > 1 and strides[-1] != 1:
         mask = mask.contiguous()
         keep.append(mask)
-    m = 1 if dim == 1 else mask.size(0)
+        strides = mask.stride()
+    m = 1 if dim == 1 else shape[0]
     if mask_index is None and m != 1 and m != n:
         raise ValueError(f"mask has {m} rows for {n} rows of logits and no mask_index")
-    return mask.data_ptr() or 1 << 12, (0 if dim == 1 else mask.stride(0)), m, \
-        _per_row(mask_index, n, dev, torch.int32, "mask_index", keep)
+    index = 0 if mask_index is None else _per_row(mask_index, n, dev, torch.int32, "mask_index", keep)
+    return mask.data_ptr() or 1 << 12, (0 if dim == 1 else strides[0]), m, index
 
 
 def _call(name: str, dev: int, status: Optional[torch.Tensor], *args) -> None:
@@ -128,13 +134,12 @@ def _call(name: str, dev: int, status: Optional[torch.Tensor], *args) -> None:
     elif status.dtype is not torch.int32 or status.get_device() != dev or status.numel() < 1:
         raise ValueError(f"status must be an int32 tensor on cuda:{dev}")
     stream = _device_stream(dev)
-    handle = lib()
-    st = getattr(handle, name)(*args, status.data_ptr(), stream)
+    st = getattr(lib(), name)(*args, status.data_ptr(), stream)
     if st:
         check(st, name)
     if own:
         word = C.c_int(0)
-        check(handle.cnnue_read_status(status.data_ptr(), stream, C.byref(word)), "cnnue_read_status")
+        check(lib().cnnue_read_status(status.data_ptr(), stream, C.byref(word)), "cnnue_read_status")
         check(word.value, f"{name} (kernel status)")
 
 
@@ -167,7 +172,7 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     CnnueError (bad index; the token is skipped), a length outside [0, L] too
     (bad offsets; clamped); with `status` (int32 device tensor) the bits are
     collected there instead and nothing synchronises.  Not differentiable."""
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("process_logits is not differentiable: detach the logits or use policy_loss")
     z = _rows(logits, "logits")
     n, vocab = z.shape
