@@ -554,9 +554,10 @@ struct LossArgs {
 
 // Exponentials are exp2(x c - B) with c = log2(e) in fp32 and B = m c rounded:
 // one fused operation per element before the instruction, and because every
-// thread and both passes take the same B for the same m, B's rounding cancels
-// in exp / sum; the loss takes it out (residual()).  |m| near fp32's limit,
-// where m c would overflow, goes through (x - m) c.
+// thread and both passes take the same B for the same m, B's rounding r = m c -
+// B cancels in exp / sum; the loss takes it out (residual()).  Above |m| = 2^16,
+// where r is no longer small (2^-8 there) and m c in the end overflows, they
+// are exp2((x - m) c), and r is 0.
 struct Sums {
   float m, s, t, d;  // maximum, sum of exp2(z c - B(m)), target mass, sum of t (m - z)
 };
@@ -566,20 +567,20 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ bool huge(float m) { return fabsf(m) > 1e38f; }  // infinities too
+__device__ __forceinline__ bool huge(float m) { return fabsf(m) > 65536.f; }  // infinities too
 __device__ __forceinline__ float base(float m) { return __fmul_rn(m, rows::kLog2e); }
+__device__ __forceinline__ float rounding(float m) { return huge(m) ? 0.f : fmaf(m, rows::kLog2e, -base(m)); }
 // exp2(z c - B(from)) times this is exp2(z c - B(to)); from -inf: 0.
 __device__ __forceinline__ float rebase(float from, float to) {
   if (from == kNegInf) return 0.f;
-  return exp2_fast(huge(from) || huge(to) ? (from - to) * rows::kLog2e : base(from) - base(to));
+  if (huge(from) || huge(to)) return exp2_fast((from - to) * rows::kLog2e - rounding(from) + rounding(to));
+  return exp2_fast(base(from) - base(to));
 }
+// log of what B's rounding put into the sum.
+__device__ __forceinline__ float residual(float m) { return 0.693147180559945309f * rounding(m); }
 // exp2(z c - B(m)) of one logit, m not -inf.
 __device__ __forceinline__ float exp_of(float z, float m) {
   return exp2_fast(huge(m) ? (z - m) * rows::kLog2e : fmaf(z, rows::kLog2e, -base(m)));
-}
-// log of what B's rounding put into the sum.
-__device__ __forceinline__ float residual(float m) {
-  return huge(m) ? 0.f : 0.693147180559945309f * fmaf(m, rows::kLog2e, -base(m));
 }
 // The sums of the warp's lanes, each relative to its own maximum, as one;
 // every lane gets the same bits.  A side without a logit above -inf has s = 0;

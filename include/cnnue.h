@@ -452,7 +452,8 @@ int cnnue_logits_process(const void* d_logits, int64_t logits_stride, int logits
  * allowed are dropped.  A row of which nothing is left (no allowed logit
  * above -inf) has loss 0 and gradient 0; so has a row of weight 0, which is
  * not read.  A NaN at an allowed token makes the row's loss and gradient NaN;
- * elsewhere it is not read.  A listed token >= vocab sets
+ * elsewhere it is not read.  M - z is formed in fp32 (infinite beyond its
+ * range).  A listed token >= vocab sets
  * CNNUE_STATUS_BAD_INDEX and is skipped.  Takes the role of the policy part
  * of compute_batch_loss (src/az/train_gpu_candle.rs:221-305). */
 typedef struct cnnue_loss_targets {

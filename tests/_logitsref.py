@@ -114,7 +114,9 @@ def loss(logits, targets=None, target_index=None, target_prob=None, mask=None, m
         m = zr.max() if not zr.isnan().any() else torch.tensor(math.nan, dtype=torch.double)
         e = torch.exp(zr - m)
         s, mass = e.sum(), tr.sum()
-        d = torch.where(tr != 0, tr * (m - zr), torch.zeros_like(zr))
+        # M - z is formed in fp32: from FLT_MAX and half a step on it is infinite (2e37 + 3.4028e38 > 3.4029e38)
+        apart = torch.where(m - zr >= 2.0 ** 128 - 2.0 ** 103, torch.full_like(zr, math.inf), m - zr)
+        d = torch.where(tr != 0, tr * apart, torch.zeros_like(zr))
         log_s = torch.log(s) if mass != 0 else torch.zeros(())
         out[r] = w[r] * (mass * log_s + d.sum())
         p = mass * e / s if mass != 0 else torch.zeros_like(e)

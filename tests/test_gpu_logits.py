@@ -418,6 +418,20 @@ def test_loss_of_a_common_offset_keeps_its_digits(dtype):
     check_all(x, {"target_index": torch.tensor([5, 0, 2085]), "mask": mask_of(3, 2086, 0.9, g) | -1}, dtype)
 
 
+@pytest.mark.parametrize("offset", [3e4, 65530.0, 1e6, -65530.0, -1e7, 1e10, -1e12, 1e20, -1e30, 2e37])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_loss_of_large_logits(offset, dtype):
+    """Logits around any size, with steps of their type's own spacing and rows that reach across sizes."""
+    g = gen(23)
+    step = abs(offset) * torch.finfo(dtype).eps
+    x = (offset + torch.randint(-3, 4, (4, 900), generator=g).double() * step).to(dtype)
+    x[1, ::3] = 0.0  # far below or above the others
+    x[2, 5:] = torch.finfo(dtype).min
+    x[3] = torch.linspace(-1, 1, 900) * 70000 if abs(offset) < 1e8 else x[3]
+    check_all(x, {"target_index": torch.tensor([[5, 7], [0, 1], [3, 899], [898, 4]]), "target_prob": torch.rand(4, 2, generator=g)},
+              dtype)
+
+
 @pytest.mark.parametrize("kind", ["dense", "labels", "lists"])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_loss_rows_where_little_or_nothing_is_left(kind, dtype):
