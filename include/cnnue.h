@@ -596,7 +596,8 @@ int cnnue_adamw_device_scaled(float* d_params, float* d_m, float* d_v, const flo
  *   (448 / max|x|)) rounded to nearest even, u' > 0 never below 2^-9 of the
  *   scale (a second moment above zero stays above zero)
  * in fp32 (u' good to 0.501 of its last place, the step's quotient to 2^-22;
- * a v' below 2^-126 gives a u' below 2^-62); the update uses m' and u' before they are rounded to 8
+ * a v' below 2^-126 gives a u' below 2^-62, one that overflows the root of
+ * fp32's largest value); the update uses m' and u' before they are rounded to 8
  * bits.  A NaN or infinity in a block's m' (u') makes the scale and the codes of that
  * block's m (u) non-finite.
  * copy (optional): the updated parameter rounded to copy_type (bf16 or fp16),

@@ -601,6 +601,25 @@ def test_results_do_not_change_from_run_to_run(dtype):
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_more_than_32_bits_apart(dtype):
+    """Elements and bytes past 2^32, of the logits, the results and the targets."""
+    g = gen(31)
+    R, V, far = 4, 20_001, (1 << 30) + 3
+    x = rows(R, V, dtype, g)
+    kw = dict(history=history_of(R, V, 100, g), frequency=torch.rand(R, generator=g), mask=mask_of(R, V, 0.5, g))
+    size = (R - 1) * far + V
+    a, b = (torch.empty(size, dtype=dtype, device=DEV).as_strided((R, V), (far, 1)) for _ in range(2))
+    a.copy_(x)
+    want, bound = ref.process(x, **kw)
+    ref.close(lg.process_logits(a, out=b, **{k: dev(t) for k, t in kw.items()}), want, bound, dtype)
+    t = torch.rand(R, V, generator=g)
+    want, grad, bl, bg = ref.loss(x, t, mask=kw["mask"])
+    loss, got = lg.policy_loss_grad(a, dev(t), mask=dev(kw["mask"]), grad=b)
+    ref.close(loss, want, bl)
+    ref.close(got, grad, bg, dtype)
+
+
 # ---- together, as they are used -----------------------------------------------------
 def test_legal_moves_choose_learn_and_update():
     """The ResNet's logits under the rules of the game: legal-move priors; then

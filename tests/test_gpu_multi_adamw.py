@@ -268,6 +268,36 @@ def test_a_block_with_a_nan_becomes_one_and_the_others_do_not():
     assert torch.isfinite(p[[0, 299, 301, 599, 601, 1023]]).all() and p[300].isnan()
 
 
+def test_gradients_whose_square_overflows():
+    """v' saturates: the step stays finite, and the rest of the block's root moments with it."""
+    g = torch.full((512,), 1e-3, device=DEV)
+    g[5] = 1e25
+    p = torch.ones(512, device=DEV)
+    opt = MultiAdamW([p], [g], state_bits=8, lr=LR, weight_decay=0.0)
+    opt.step()
+    opt.step()
+    u = opt.state["v"][0].float() * opt.state["v_scale"][0].repeat_interleave(256)
+    assert torch.isfinite(p).all() and torch.isfinite(u).all() and u[5] > 1e19
+
+
+def test_a_tensor_of_more_than_two_to_the_31_elements():
+    n, tail = 2 ** 31 + 777, 2000
+    small_p = torch.randn(tail, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    small_g = torch.randn(tail, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    off = (n - tail) % 256  # the same blocks of 256 at the end of both
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device=DEV), torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    q, h = torch.zeros(off + tail, dtype=torch.bfloat16, device=DEV), torch.zeros(off + tail, dtype=torch.bfloat16, device=DEV)
+    for t, v in ((p, small_p), (g, small_g), (q, small_p), (h, small_g)):
+        t[-tail:] = v.to(DEV)
+    for bits in (8, 32):
+        a, b = MultiAdamW([p], [g], state_bits=bits), MultiAdamW([q], [h], state_bits=bits)
+        a.step()
+        b.step()
+        assert torch.equal(p[-tail:], q[-tail:]) and not p[:4096].any()
+        assert torch.equal(a.state["m"][0][-tail:].float(), b.state["m"][0][-tail:].float())
+        del a
+
+
 def test_tiny_and_zero_blocks():
     g = torch.zeros(768, device=DEV)
     g[256:512] = 1e-38
