@@ -128,6 +128,7 @@ constexpr int kFusedTokens = 16384;  // 32 or 64 KB of counters
 constexpr int kCountThreads = 512;
 constexpr int kTokensAhead = 4;  // history tokens per thread that are read first of all,
 constexpr int kMoreTokens = 8;   // and after those, in flight
+constexpr int64_t kMostTokens = 0x7fff0000;  // longest history (its positions plus a round of a CTA fit 31 bits)
 constexpr int kHashTokens = kCountThreads * kTokensAhead;  // the longest history that is counted in a hash table
 
 struct ProcArgs {
@@ -234,7 +235,7 @@ struct Table {
   // Counts the tokens in slots s[0..N) (negative: none) at positions i, i +
   // stride, ..; bit j of the result: s[j] had not occurred.
   template <int N>
-  __device__ __forceinline__ uint32_t see(const int* s, int64_t i, int stride, int64_t prompt) const {
+  __device__ __forceinline__ uint32_t see(const int* s, int i, int stride, int prompt) const {
     uint32_t before[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -302,17 +303,18 @@ __device__ __forceinline__ void penalise(const ProcArgs& a, const TI* in, TO* ou
   const bool hist = a.r.history != nullptr, bias = a.r.bias_tokens != nullptr;
   const Table<BITS, HASH> table(smem, &listed, a.slots, a.lg, bias);
   Penalties pen;
-  int64_t len = 0, prompt = 0;
+  const int most = hist ? (int)a.r.history_len : 0;  // below kMostTokens: positions are 32-bit
+  int len = most, prompt = 0;
   const bool wide = a.r.history_bytes == 8;
   const char* list = (const char*)a.r.history + row * a.r.history_stride * a.r.history_bytes;
   int ahead[kTokensAhead];
 #pragma unroll
   for (int j = 0; j < kTokensAhead; ++j) {
-    const int64_t i = threadIdx.x + j * stride;
-    ahead[j] = hist && i < a.r.history_len ? rows::token_at(list, i, wide) : -1;
+    const int i = threadIdx.x + j * stride;
+    ahead[j] = i < most ? rows::token_at(list, i, wide) : -1;
   }
   if (hist) {
-    len = a.r.lengths ? (int64_t)a.r.lengths[row] : a.r.history_len;
+    if (a.r.lengths) len = a.r.lengths[row];
     if (a.r.prompt_lengths) prompt = a.r.prompt_lengths[row];
     if (a.r.repetition) pen.rep = a.r.repetition[row];
     if (a.r.frequency) pen.freq = a.r.frequency[row];
@@ -331,13 +333,13 @@ __device__ __forceinline__ void penalise(const ProcArgs& a, const TI* in, TO* ou
   auto value = [&](int t) { return Vec<TI>::up(in[t]); };
   float x[kTokensAhead], x_biased = 0.f;
   uint32_t mine = 0, stays = 0;  // bit j: token j is this thread's to compute; the mask allows it
-  if (len < 0 || len > a.r.history_len) {
-    if (hist && threadIdx.x == 0 && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_OFFSETS);
-    len = max((int64_t)0, min(len, a.r.history_len));
+  if (len < 0 || len > most) {
+    if (threadIdx.x == 0 && part == 0) atomicOr(a.status, CNNUE_STATUS_BAD_OFFSETS);
+    len = max(0, min(len, most));
   }
 #pragma unroll
   for (int j = 0; j < kTokensAhead; ++j) {
-    ahead[j] = threadIdx.x + j * stride < len ? own(ahead[j]) : -1;
+    ahead[j] = (int)threadIdx.x + j * stride < len ? own(ahead[j]) : -1;
     x[j] = ahead[j] >= 0 ? value(ahead[j]) : 0.f;
     if (ahead[j] >= 0 && token_ok(mask, ahead[j])) stays |= 1u << j;
   }
@@ -351,8 +353,8 @@ __device__ __forceinline__ void penalise(const ProcArgs& a, const TI* in, TO* ou
   for (int j = 0; j < kTokensAhead; ++j) at[j] = ahead[j] >= 0 ? table.slot(ahead[j]) : -1;
   mine = table.template see<kTokensAhead>(at, threadIdx.x, stride, prompt);
   if (!HASH) {  // a hash table's histories end here
-    for (int64_t b = kTokensAhead * stride; b < len; b += kMoreTokens * stride) {  // the same for all threads
-      const int64_t i = b + threadIdx.x;
+    for (int b = kTokensAhead * stride; b < len; b += kMoreTokens * stride) {  // the same for all threads
+      const int i = b + threadIdx.x;
       int s[kMoreTokens];
 #pragma unroll
       for (int j = 0; j < kMoreTokens; ++j) s[j] = i + j * stride < len ? rows::token_at(list, i + j * stride, wide) : -1;
@@ -1216,7 +1218,7 @@ int cnnue_logits_process(const void* d_logits, int64_t logits_stride, int logits
   const cnnue_logit_rules& r = *rules;
   if (r.history) {
     if (r.history_bytes != 4 && r.history_bytes != 8) return set_error(CNNUE_ERR_INVALID_ARG, "history_bytes");
-    if (r.history_len < 0 || r.history_len > 0x7fffffff || r.history_stride < 0)
+    if (r.history_len < 0 || r.history_len > kMostTokens || r.history_stride < 0)
       return set_error(CNNUE_ERR_INVALID_ARG, "history: length or stride");
   } else if (r.repetition || r.frequency || r.presence || r.lengths || r.prompt_lengths) {
     return set_error(CNNUE_ERR_INVALID_ARG, "penalties without a history");
