@@ -593,6 +593,8 @@ class AzTrainer:
         the word as a float.  adamw=True also applies AdamW (single GPU): the
         table leaves' update runs while the dense gradients finish."""
         torch = self.torch
+        if adamw and self.optimizer is not None:
+            raise ValueError("adamw=True is the 32-bit form; with state_bits=8 call optimizer.step()")
         bt = self.expand(bt)
         B, F = bt["feature_items"].shape
         M = bt["policy_items"].shape[1]

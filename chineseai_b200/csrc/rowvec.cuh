@@ -191,27 +191,6 @@ __device__ __forceinline__ uint32_t allowed_whole(const uint32_t* __restrict__ m
   return b & kFull<VE>;
 }
 
-// The elements of vector e0 that `want` names (a subset of inside()); the
-// others get `rest`.
-template <typename T>
-__device__ __forceinline__ void load(const T* row, int e0, uint32_t in, uint32_t want, float rest, float* x) {
-  constexpr int VE = Vec<T>::VE;
-  if (want == 0) {
-#pragma unroll
-    for (int i = 0; i < VE; ++i) x[i] = rest;
-    return;
-  }
-  if (in == kFull<VE>) {
-    Vec<T>::unpack(load16(row + e0), x);
-#pragma unroll
-    for (int i = 0; i < VE; ++i)
-      if (!(want >> i & 1)) x[i] = rest;
-  } else {
-#pragma unroll
-    for (int i = 0; i < VE; ++i) x[i] = want >> i & 1 ? Vec<T>::up(row[e0 + i]) : rest;
-  }
-}
-
 // The raw vector e0 with at least the elements of `want` in it (the others are
 // whatever a whole load brings, or 0).
 template <typename T>

@@ -372,6 +372,9 @@ def test_az_trainer_with_8_bit_states(native, graph):
     with pytest.raises(CnnueError):
         b.step(bad)
     assert torch.equal(b.flat, before) and b.optimizer.step_count == 4
+    if native:
+        with pytest.raises(ValueError, match="state_bits"):
+            b.native_loss(b.to_device(batch), adamw=True)
     b.set_learning_rate(0.0)
     b.step(batch)
     assert torch.equal(b.flat, before * 1.0) and b.optimizer.step_count == 5
