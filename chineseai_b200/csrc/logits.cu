@@ -1085,6 +1085,12 @@ int launch_loss(const LossArgs& a, int threads, cudaStream_t s) {
 // 131072 bf16: 117 us with 4 CTAs of 64 KB per row, 139 with 8 of 32 KB (twice
 // the threads' fixed work, and more to wait for in each cluster).
 constexpr int kSliceVectors = 4096;
+// Longer rows keep slices of up to 100 KB, 2 CTAs per SM (400 x 200000 fp32:
+// 152 us, 196 read twice).  Above that one CTA fills an SM: slower than reading
+// twice when the clusters take turns (dense 16 x 262144 fp32: 107 us, 87; 600
+// rows: 428, 338), faster while all run at once (14 rows: 66 us, 87), which 14
+// clusters of 8 do; up to 192 KB.
+constexpr int kKeepVectors = 6400, kKeepAlone = 12288, kAloneCtas = 112;
 
 template <typename T, bool GRAD>
 int run_loss(LossArgs a, cudaStream_t s) {
@@ -1097,7 +1103,7 @@ int run_loss(LossArgs a, cudaStream_t s) {
   // with 8), 8 for more rows, where the threads' fixed work counts (16384 x 2086 fp32: 66 us, 82 with 4).
   const int per = a.n_rows * ctas > 148 * 8 ? 8 : 4;
   const int threads = (int)std::min<int64_t>(kLossThreads, std::max<int64_t>(1, a.vps / (per * 32)) * 32);
-  if (GRAD && a.vps <= kSliceVectors)
+  if (GRAD && a.vps <= (a.n_rows * ctas <= kAloneCtas ? kKeepAlone : kKeepVectors))
     return a.t.dense ? launch_loss<T, GRAD, GRAD, true>(a, threads, s) : launch_loss<T, GRAD, GRAD, false>(a, threads, s);
   return a.t.dense ? launch_loss<T, false, GRAD, true>(a, threads, s) : launch_loss<T, false, GRAD, false>(a, threads, s);
 }

@@ -390,6 +390,21 @@ def test_loss_large_vocabulary(dtype):
     check_all(x, kw, dtype)
 
 
+@pytest.mark.parametrize("kind", ["dense", "labels"])
+@pytest.mark.parametrize("size", [(2, 190_003), (20, 190_003), (2, 260_000), (20, 260_000), (1, 400_001), (1, 1_000_003)])
+def test_loss_of_rows_kept_or_read_twice(size, kind):
+    """fp32 rows at both sides of each limit of what a cluster keeps, few and many of them."""
+    g = gen(size[1])
+    x, kw = loss_inputs(*size, torch.float32, kind, g)
+    d = {k: dev(t) for k, t in kw.items()}
+    targets = d.pop("targets", None)
+    loss, got = lg.policy_loss_grad(dev(x), targets, **d)
+    one = slice(size[0] - 1, size[0])
+    want, grad, bl, bg = ref.loss(x[one], **{k: t[one] for k, t in kw.items()})
+    ref.close(loss[one], want, bl)
+    ref.close(got[one], grad, bg)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("pad,offset", [(0, 1), (3, 0), (5, 3)])
 def test_loss_strides_and_neighbours(pad, offset, dtype):
