@@ -129,6 +129,7 @@ constexpr int kCountThreads = 512;
 constexpr int kTokensAhead = 4;  // history tokens per thread that are read first of all,
 constexpr int kMoreTokens = 8;   // and after those, in flight
 constexpr int64_t kMostTokens = 0x7fff0000;  // longest history (its positions plus a round of a CTA fit 31 bits)
+constexpr int kCountBytes = 144 * 1024;  // the largest Table
 constexpr int kHashTokens = kCountThreads * kTokensAhead;  // the longest history that is counted in a hash table
 
 struct ProcArgs {
@@ -452,12 +453,20 @@ __global__ void __launch_bounds__(kCountThreads, 2) penalise_kernel(const __grid
                                [] { asm volatile("griddepcontrol.wait;" ::: "memory"); });
 }
 
+// Lets a kernel have more than 48 KB of shared memory: always `most`, so that
+// calls of other sizes in other threads never set a lower limit in between.
+template <typename F>
+int allow_smem(F* kernel, size_t smem, int most) {
+  if (smem > (size_t)most) return set_error(CNNUE_ERR_INVALID_ARG, "%zu bytes of shared memory", smem);
+  if (smem > 40 * 1024) CNNUE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+  return CNNUE_OK;
+}
+
 template <typename F>
 int launch_process(F* kernel, const ProcArgs& a, int64_t blocks, int threads, size_t smem, bool dependent, cudaStream_t s,
                    const char* what) {
   if (blocks > 0x7fffffff) return set_error(CNNUE_ERR_INVALID_ARG, "too many rows for one call");
-  if (smem > 40 * 1024)
-    CNNUE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (int st = allow_smem(kernel, smem, kCountBytes)) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3((unsigned)threads);
@@ -1061,26 +1070,6 @@ __global__ void __launch_bounds__(kLossThreads) loss_bwd_kernel(const LossArgs a
   }
 }
 
-template <typename T, bool KEEP, bool GRAD, bool DENSE>
-int launch_loss(const LossArgs& a, int threads, cudaStream_t s) {
-  if (a.n_rows * a.split > 0x7fffffff) return set_error(CNNUE_ERR_INVALID_ARG, "too many rows for one call");
-  auto* kernel = loss_kernel<T, KEEP, GRAD, DENSE>;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.n_rows * a.split));
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = KEEP ? (size_t)a.vps * 16 : 0;
-  cfg.stream = s;
-  if (cfg.dynamicSmemBytes > 40 * 1024)
-    CNNUE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes));
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim = {(unsigned)a.split, 1, 1};
-  cfg.attrs = &attr;
-  cfg.numAttrs = a.split > 1 ? 1 : 0;
-  CNNUE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
-  return check_launch_error("loss_kernel");
-}
-
 // A slice is at most 64 KB of shared memory, 3 CTAs per SM.  Measured at 1024 x
 // 131072 bf16: 117 us with 4 CTAs of 64 KB per row, 139 with 8 of 32 KB (twice
 // the threads' fixed work, and more to wait for in each cluster).
@@ -1091,6 +1080,25 @@ constexpr int kSliceVectors = 4096;
 // rows: 428, 338), faster while all run at once (14 rows: 66 us, 87), which 14
 // clusters of 8 do; up to 192 KB.
 constexpr int kKeepVectors = 6400, kKeepAlone = 12288, kAloneCtas = 112;
+
+template <typename T, bool KEEP, bool GRAD, bool DENSE>
+int launch_loss(const LossArgs& a, int threads, cudaStream_t s) {
+  if (a.n_rows * a.split > 0x7fffffff) return set_error(CNNUE_ERR_INVALID_ARG, "too many rows for one call");
+  auto* kernel = loss_kernel<T, KEEP, GRAD, DENSE>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.n_rows * a.split));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = KEEP ? (size_t)a.vps * 16 : 0;
+  cfg.stream = s;
+  if (int st = allow_smem(kernel, cfg.dynamicSmemBytes, kKeepAlone * 16)) return st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {(unsigned)a.split, 1, 1};
+  cfg.attrs = &attr;
+  cfg.numAttrs = a.split > 1 ? 1 : 0;
+  CNNUE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
+  return check_launch_error("loss_kernel");
+}
 
 template <typename T, bool GRAD>
 int run_loss(LossArgs a, cudaStream_t s) {

@@ -2,6 +2,7 @@
 (tests/_logitsref.py), at the sizes, types, strides and masks where rows,
 slices and vectors end."""
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -686,3 +687,41 @@ def test_legal_moves_choose_learn_and_update():
         # below 2^-60 the squares leave fp32's normal range and the root loses digits
         big = (g64.abs() > 2.0 ** -55) | (g64 == 0)
         assert ((q.cpu().double() - step).abs()[big] <= 16 * ref.EPS32 * (step.abs() + 1e-2)[big]).all()
+
+
+def test_calls_of_other_sizes_in_other_threads():
+    """Calls in several threads that need different amounts of shared memory give what they give alone."""
+    def jobs(seed):
+        g = gen(seed)
+        made = []
+        for vocab in (8_192, 60_001, 126_000, 190_000):
+            x = dev(torch.randn(3, vocab, generator=g))
+            label = dev(torch.randint(0, vocab, (3,), generator=g))
+            history = dev(torch.randint(0, vocab, (3, 3000), generator=g, dtype=torch.int32))
+            rule = dict(history=history, frequency=dev(torch.full((3,), 0.25)))
+            status = torch.zeros(1, dtype=torch.int32, device="cuda")
+            made.append((lambda x=x, label=label, status=status: lg.policy_loss_grad(x, target_index=label, status=status)[1]))
+            made.append((lambda x=x, rule=rule, status=status: lg.process_logits(x, **rule, status=status)))
+        return made
+
+    work = [jobs(seed) for seed in range(4)]
+    alone = [[f() for f in fs] for fs in work]
+    torch.cuda.synchronize()
+    faults = []
+
+    def run(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(50):
+                    j = (i * (2 * k + 1) + k) % len(work[k])
+                    if not torch.equal(work[k][j](), alone[k][j]):
+                        faults.append((k, j))
+        except Exception as e:  # noqa: BLE001
+            faults.append((k, repr(e)))
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(len(work))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not faults and not any(t.is_alive() for t in threads)
