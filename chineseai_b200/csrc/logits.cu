@@ -595,14 +595,15 @@ __device__ __forceinline__ float exp_of(float z, float m) {
 }
 // The sums of the warp's lanes, each relative to its own maximum, as one;
 // every lane gets the same bits.  A side without a logit above -inf has s = 0;
-// mass that sits on its -inf logits makes d infinite, as t (m - z) says.
+// mass that sits on its -inf logits makes d infinite, as t (m - z) says.  Masses
+// that cancel (t = 0) leave d as it is: a sum of signed terms, not 0.
 // TARGETS: t and d too (otherwise they are 0 in every lane).
 __device__ __forceinline__ Sums join_lanes(Sums v, bool targets) {
   float m;
   asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v.m));
   if (m != kNegInf) {
     v.s *= rebase(v.m, m);
-    if (targets) v.d = v.t != 0.f ? v.d + v.t * (m - v.m) : 0.f;
+    if (targets && v.t != 0.f) v.d += v.t * (m - v.m);
   }
   v.m = m;
 #pragma unroll
@@ -621,7 +622,7 @@ __device__ __forceinline__ void join_two(Sums& a, const Sums& b) {
   const float m = rows::max_nan(a.m, b.m);
   if (m != kNegInf) {
     a.s = a.s * rebase(a.m, m) + b.s * rebase(b.m, m);
-    a.d = (a.t != 0.f ? a.d + a.t * (m - a.m) : 0.f) + (b.t != 0.f ? b.d + b.t * (m - b.m) : 0.f);
+    a.d += b.d + (a.t != 0.f ? a.t * (m - a.m) : 0.f) + (b.t != 0.f ? b.t * (m - b.m) : 0.f);
   }
   a.t += b.t;
   a.m = m;
@@ -858,7 +859,7 @@ __device__ __forceinline__ Sums slice_sums(const LossRow<T>& r, const Slice<Vec<
       const float f = rebase(v.m, m);
       sum.x *= f;
       sum.y *= f;
-      v.d = v.t != 0.f ? v.d + v.t * (m - v.m) : 0.f;
+      if (v.t != 0.f) v.d += v.t * (m - v.m);
       v.m = m;
     }
     const float from = v.m == kNegInf ? 0.f : v.m;  // -inf - -inf would be a NaN

@@ -1,0 +1,54 @@
+"""The masked policy loss and process_logits where single targets, NaNs and
+arguments are unusual: signed targets, NaNs that few threads see, rows without
+target mass, histories without penalties; against the plain 64-bit forms."""
+import math
+
+import pytest
+import torch
+
+from tests import _logitsref as ref
+from tests.test_gpu_logits import DEV, TYPES, check_all, dev, gen
+from chineseai_b200 import logits as lg
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- targets of both signs --------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [100, 2086, 131_072])
+@pytest.mark.parametrize("kind", ["lists", "dense"])
+def test_loss_of_targets_that_cancel(kind, vocab, dtype):
+    """+p and -p in one vector, one warp, two warps, two CTAs of a cluster; alone, and beside other targets."""
+    g = gen(vocab)
+    pairs = [(4, 5), (0, vocab - 1), (8, vocab // 2), (vocab // 3, vocab // 3 + 9), (5, 9), (1, 96)]
+    x = (torch.randn(2 * len(pairs), vocab, generator=g) * 3).to(dtype)
+    K = 300  # entries of a list: the second of a pair is another warp's
+    index = torch.full((len(x), K), -1, dtype=torch.int64)
+    prob = torch.zeros(len(x), K)
+    for r, (a, b) in enumerate(pairs * 2):
+        at = (0, 1) if r % 2 else (3, 290)
+        index[r, at[0]], index[r, at[1]] = a, b
+        prob[r, at[0]], prob[r, at[1]] = 0.75, -0.75
+        if r >= len(pairs):
+            index[r, 100], prob[r, 100] = vocab // 2 + 1, 0.5
+    if kind == "lists":
+        return check_all(x, dict(target_index=index, target_prob=prob), dtype)
+    targets = torch.zeros(len(x), vocab).scatter_add_(1, index.clamp(min=0), torch.where(index >= 0, prob, 0.0))
+    check_all(x, dict(targets=targets), dtype)
+
+
+def test_loss_of_a_pair_at_any_two_tokens():
+    """A preference pair is the difference of two logits, wherever its tokens lie."""
+    g = gen(3)
+    V = 2086
+    x = torch.randn(64, V, generator=g)
+    pair = torch.stack([torch.randperm(V, generator=g)[:2] for _ in range(64)])
+    pair[0] = torch.tensor([5, 9])
+    prob = torch.tensor([1.0, -1.0]).expand(64, 2)
+    check_all(x, dict(target_index=pair, target_prob=prob), torch.float32)
+    loss, _ = lg.policy_loss_grad(dev(x), target_index=dev(pair), target_prob=dev(prob))
+    z = x.double().gather(1, pair)
+    d = z[:, 1] - z[:, 0]
+    # every value on the way is below 10; a target's difference is rounded once, in each of two joins it is moved to
+    # the joint maximum (two roundings) and added up (at most four that round)
+    assert ((loss.cpu().double() - d).abs() <= 2 * 13 * ref.EPS32 * 10).all()
