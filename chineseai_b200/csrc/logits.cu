@@ -593,17 +593,21 @@ __device__ __forceinline__ float residual(float m) { return 0.693147180559945309
 __device__ __forceinline__ float exp_of(float z, float m) {
   return exp2_fast(huge(m) ? (z - m) * rows::kLog2e : fmaf(z, rows::kLog2e, -base(m)));
 }
+// What a move of the maximum to m, not -inf, adds to d.  Masses that cancel (t =
+// 0) leave d as it is: a sum of signed terms, not 0.  So do those of a side
+// without a logit above -inf: each is t inf there already, as t (m - z) says.
+__device__ __forceinline__ float moved(const Sums& v, float m) {
+  return v.t != 0.f && v.m != kNegInf ? v.t * (m - v.m) : 0.f;
+}
 // The sums of the warp's lanes, each relative to its own maximum, as one;
-// every lane gets the same bits.  A side without a logit above -inf has s = 0;
-// mass that sits on its -inf logits makes d infinite, as t (m - z) says.  Masses
-// that cancel (t = 0) leave d as it is: a sum of signed terms, not 0.
+// every lane gets the same bits.  A side without a logit above -inf has s = 0.
 // TARGETS: t and d too (otherwise they are 0 in every lane).
 __device__ __forceinline__ Sums join_lanes(Sums v, bool targets) {
   float m;
   asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v.m));
   if (m != kNegInf) {
     v.s *= rebase(v.m, m);
-    if (targets && v.t != 0.f) v.d += v.t * (m - v.m);
+    if (targets) v.d += moved(v, m);
   }
   v.m = m;
 #pragma unroll
@@ -622,7 +626,7 @@ __device__ __forceinline__ void join_two(Sums& a, const Sums& b) {
   const float m = rows::max_nan(a.m, b.m);
   if (m != kNegInf) {
     a.s = a.s * rebase(a.m, m) + b.s * rebase(b.m, m);
-    a.d += b.d + (a.t != 0.f ? a.t * (m - a.m) : 0.f) + (b.t != 0.f ? b.t * (m - b.m) : 0.f);
+    a.d += b.d + moved(a, m) + moved(b, m);
   }
   a.t += b.t;
   a.m = m;
@@ -738,12 +742,9 @@ struct LossRow {
       if (t == 0.f) continue;
       const float x = Vec<T>::up(z[tok]);
       // relative to this thread's own maximum, which need not be above x
-      if (v.m == kNegInf && x != kNegInf) {
-        v.m = x;  // s = 0
-        v.d = v.t != 0.f ? -kNegInf : 0.f;
-      }
+      if (v.m == kNegInf) v.m = x;  // s = 0
       v.t += t;
-      v.d += v.m == kNegInf ? 0.f : t * (v.m - x);
+      v.d += t * ((v.m == kNegInf ? 0.f : v.m) - x);  // t inf on a logit of -inf
     }
   }
 
@@ -859,7 +860,7 @@ __device__ __forceinline__ Sums slice_sums(const LossRow<T>& r, const Slice<Vec<
       const float f = rebase(v.m, m);
       sum.x *= f;
       sum.y *= f;
-      if (v.t != 0.f) v.d += v.t * (m - v.m);
+      v.d += moved(v, m);
       v.m = m;
     }
     const float from = v.m == kNegInf ? 0.f : v.m;  // -inf - -inf would be a NaN
@@ -873,7 +874,7 @@ __device__ __forceinline__ Sums slice_sums(const LossRow<T>& r, const Slice<Vec<
 #pragma unroll
         for (int k = 0; k < VE; ++k) {
           v.t += t[k];
-          if (t[k] != 0.f && v.m != kNegInf) v.d += t[k] * (v.m - x[k]);
+          if (t[k] != 0.f) v.d += t[k] * (from - x[k]);
         }
       }
       exps<VE>(x, from, &sum);

@@ -52,3 +52,31 @@ def test_loss_of_a_pair_at_any_two_tokens():
     # every value on the way is below 10; a target's difference is rounded once, in each of two joins it is moved to
     # the joint maximum (two roundings) and added up (at most four that round)
     assert ((loss.cpu().double() - d).abs() <= 2 * 13 * ref.EPS32 * 10).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["lists", "dense"])
+def test_loss_of_targets_on_minus_infinity(kind, dtype):
+    """t (M - z) there is an infinity of the target's sign, whichever thread meets it, before or after a finite logit;
+    infinities of both signs are NaN."""
+    g = gen(17)
+    V, R, K = 2086, 12, 300
+    x = torch.randn(R, V, generator=g).to(dtype)
+    x[:, 4:2000] = x[:, 2008:] = -math.inf  # most threads see nothing else
+    index = torch.full((R, K), -1, dtype=torch.int64)
+    prob = torch.zeros(R, K)
+    for r in range(R):
+        sign = -1.0 if r % 2 else 1.0
+        token = (100, 700, 1499)[r % 3]
+        entry, finite = ((26, 282), (282, 26), (40, 41))[r // 2 % 3]  # a thread's first or second entry, another thread's
+        index[r, entry], prob[r, entry] = token, sign * 0.5
+        index[r, finite], prob[r, finite] = (2000, 3)[r % 2], 1.0
+    index[10, 100], prob[10, 100] = 101, -prob[10, index[10] >= 100].max()
+    index[11, 0:2], prob[11, 0:2] = torch.tensor([600, 601]), torch.tensor([0.5, -0.25])
+    if kind == "lists":
+        kw = dict(target_index=index, target_prob=prob)
+    else:
+        kw = dict(targets=torch.zeros(R, V).scatter_add_(1, index.clamp(min=0), torch.where(index >= 0, prob, 0.0)))
+    want = ref.loss(x, **kw)[0]
+    assert torch.isinf(want[:10]).all() and (want[:10] < 0).any() and want[10:].isnan().all()
+    check_all(x, kw, dtype)
