@@ -857,6 +857,7 @@ __device__ __forceinline__ Sums slice_sums(const LossRow<T>& r, const Slice<Vec<
 #pragma unroll
     for (int j = 1; j < N; ++j) m = rows::max_nan(m, Vec<T>::top(raw[j]));
     if (!(m <= v.m)) {  // a new maximum, or a NaN: what is summed so far relative to it
+      m = rows::max_nan(m, v.m);  // a NaN stays one, whatever follows it
       const float f = rebase(v.m, m);
       sum.x *= f;
       sum.y *= f;

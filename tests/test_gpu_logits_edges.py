@@ -80,3 +80,46 @@ def test_loss_of_targets_on_minus_infinity(kind, dtype):
     want = ref.loss(x, **kw)[0]
     assert torch.isinf(want[:10]).all() and (want[:10] < 0).any() and want[10:].isnan().all()
     check_all(x, kw, dtype)
+
+
+# ---- NaNs at allowed tokens ---------------------------------------------------------
+def check_nan_rows(x, a, kw, dtype):
+    """Every row of x is NaN: its loss, and its gradient at the allowed tokens; 0 at the others."""
+    d = {k: dev(t) for k, t in kw.items()}
+    targets = d.pop("targets", None)
+    loss, got = lg.policy_loss_grad(dev(x), targets, **d)
+    leaf = dev(x).requires_grad_(True)
+    again = lg.policy_loss(leaf, targets, **d)
+    again.sum().backward()
+    for rows, grad in ((loss, got), (again, leaf.grad)):
+        assert rows.isnan().all(), rows
+        assert torch.equal(grad.isnan().cpu(), a) and not grad.cpu()[~a].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["dense", "labels", "lists"])
+@pytest.mark.parametrize("rows,vocab", [(1, 64), (3, 2086), (1, 8100), (2, 50_001), (3, 131_072), (1, 900_001)])
+@pytest.mark.parametrize("hidden", ["mask", "-inf"])
+def test_loss_keeps_a_nan_that_nothing_finite_follows(hidden, rows, vocab, kind, dtype):
+    """One allowed token, a NaN, among masked ones or logits of -inf: at the row's start, where the thread that meets it
+    has all its other vectors to go, in the middle and at the end; one CTA and clusters, rows kept and read twice."""
+    g = gen(vocab)
+    for at in (5, vocab // 2, vocab - 1):
+        x = torch.randn(rows, vocab, generator=g).to(dtype)
+        a = torch.ones(rows, vocab, dtype=torch.bool)
+        kw = {}
+        if hidden == "mask":
+            a[:] = False
+            a[:, at] = True
+            kw["mask"] = lg.pack_mask(a)
+        else:
+            x[:] = -math.inf
+        x[:, at] = math.nan
+        if kind == "dense":
+            kw["targets"] = torch.rand(rows, vocab, generator=g)
+        elif kind == "labels":
+            kw["target_index"] = torch.full((rows,), at)
+        else:
+            kw["target_index"] = torch.tensor([[-1, at, at, 0]]).expand(rows, 4).contiguous()
+            kw["target_prob"] = torch.tensor([[1.0, 0.5, 0.25, 0.125]]).expand(rows, 4).contiguous()
+        check_nan_rows(x, a, kw, dtype)
