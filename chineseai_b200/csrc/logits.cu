@@ -1004,7 +1004,7 @@ __global__ void __launch_bounds__(kLossThreads, 4) loss_kernel(const __grid_cons
   }
   const bool none = v.m == kNegInf;  // nothing is left of the row
   if (rank == 0 && threadIdx.x == 0) {
-    if (a.loss) a.loss[row] = none ? 0.f : w * ((v.t != 0.f ? v.t * (logf(v.s) - residual(v.m)) : 0.f) + v.d);
+    if (a.loss) a.loss[row] = none ? 0.f : w * (v.t * (logf(v.s) - residual(v.m)) + v.d);
     if (a.stats) {
       a.stats[3 * row] = v.m;
       a.stats[3 * row + 1] = v.s;
@@ -1013,7 +1013,7 @@ __global__ void __launch_bounds__(kLossThreads, 4) loss_kernel(const __grid_cons
   }
   if (GRAD) {
     T* g = (T*)a.grad + row * a.grad_stride;
-    const float c = none || v.t == 0.f ? 0.f : __fdividef(w * v.t, v.s);
+    const float c = none ? 0.f : __fdividef(w * v.t, v.s);  // without target mass 0, or a NaN that s holds
     slice_grads<T, KEEP, DENSE>(r, slice, kept, g, v, none, c, w);
     if (!DENSE && !none) {
       __syncthreads();  // the listed tokens' elements again, now with their targets
@@ -1034,7 +1034,7 @@ __global__ void __launch_bounds__(kLossThreads) loss_bwd_kernel(const LossArgs a
   const float m = a.stats[3 * r.row], s = a.stats[3 * r.row + 1], mass = a.stats[3 * r.row + 2];
   const bool none = w == 0.f || m == kNegInf;
   if (a.upstream) w *= a.upstream[r.row];
-  const float c = none || mass == 0.f ? 0.f : w * mass / s;
+  const float c = none ? 0.f : w * mass / s;
   const Slice<VE> slice(rank, a.vps, r.shift, a.vocab);
   __shared__ Repeats repeats;
   if (!DENSE && !none && a.t.count > 1) {

@@ -123,3 +123,32 @@ def test_loss_keeps_a_nan_that_nothing_finite_follows(hidden, rows, vocab, kind,
             kw["target_index"] = torch.tensor([[-1, at, at, 0]]).expand(rows, 4).contiguous()
             kw["target_prob"] = torch.tensor([[1.0, 0.5, 0.25, 0.125]]).expand(rows, 4).contiguous()
         check_nan_rows(x, a, kw, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [100, 2086, 131_072, 900_001])
+@pytest.mark.parametrize("kind", ["dense", "lists", "labels"])
+def test_loss_of_a_nan_row_without_target_mass(kind, vocab, dtype):
+    """No target at all, targets on masked tokens only, masses that cancel: the NaN is there all the same."""
+    g = gen(vocab + 1)
+    R = 6
+    x = torch.randn(R, vocab, generator=g).to(dtype)
+    x[:3, vocab // 3] = math.nan  # among finite logits
+    x[3:] = -math.inf  # alone
+    x[3:, 7] = math.nan
+    a = torch.rand(R, vocab, generator=g) < 0.7
+    a[:, :20] = a[:, vocab // 3] = True
+    a[:, 20] = False
+    index = torch.tensor([[-1, -1, -1], [20, 20, -1], [4, 9, -1]]).repeat(2, 1)  # nothing, masked, +0.5 and -0.5
+    prob = torch.tensor([0.5, -0.5, 1.0]).expand(R, 3)
+    if kind == "lists":
+        kw = dict(target_index=index, target_prob=prob)
+    elif kind == "labels":
+        kw = dict(target_index=torch.tensor([-1, 20, -1, 20, -1, 9]))  # the last has its mass on another token
+    else:
+        kw = dict(targets=torch.zeros(R, vocab).scatter_add_(1, index.clamp(min=0), torch.where(index >= 0, prob, 0.0)))
+    check_nan_rows(x, a, dict(kw, mask=lg.pack_mask(a)), dtype)
+    idle = dict(kw, mask=lg.pack_mask(a), weights=torch.zeros(R))  # rows of weight 0 are not read
+    d = {k: dev(t) for k, t in idle.items()}
+    loss, got = lg.policy_loss_grad(dev(x), d.pop("targets", None), **d)
+    assert not loss.any() and not got.any()
