@@ -1013,7 +1013,7 @@ __global__ void __launch_bounds__(kLossThreads, 4) loss_kernel(const __grid_cons
   }
   if (GRAD) {
     T* g = (T*)a.grad + row * a.grad_stride;
-    const float c = none ? 0.f : __fdividef(w * v.t, v.s);  // without target mass 0, or a NaN that s holds
+    const float c = none ? 0.f : w * v.t / v.s;  // without target mass 0, or a NaN that s holds
     slice_grads<T, KEEP, DENSE>(r, slice, kept, g, v, none, c, w);
     if (!DENSE && !none) {
       __syncthreads();  // the listed tokens' elements again, now with their targets

@@ -152,3 +152,16 @@ def test_loss_of_a_nan_row_without_target_mass(kind, vocab, dtype):
     d = {k: dev(t) for k, t in idle.items()}
     loss, got = lg.policy_loss_grad(dev(x), d.pop("targets", None), **d)
     assert not loss.any() and not got.any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(200, 100), (33, 2086), (5, 131_072), (2, 500_009)])
+def test_loss_both_forms_give_the_same_bits(rows, vocab, dtype):
+    g = gen(vocab + 2)
+    x = dev((torch.randn(rows, vocab, generator=g) * 3).to(dtype)).requires_grad_(True)
+    kw = dict(target_index=dev(torch.randint(0, vocab, (rows, 5), generator=g)), target_prob=dev(torch.rand(rows, 5, generator=g)),
+              weights=dev(torch.rand(rows, generator=g)))
+    loss, grad = lg.policy_loss_grad(x.detach(), **kw)
+    again = lg.policy_loss(x, **kw)
+    again.sum().backward()
+    assert torch.equal(loss, again) and torch.equal(grad, x.grad)
