@@ -264,8 +264,9 @@ def _refuse_gradients(*tensors) -> None:
             raise ValueError("targets, target_prob and weights: the loss is differentiable in the logits only")
 
 
-def _addresses(tensors) -> list:
-    return [0 if x is None else x.data_ptr() for x in tensors]
+def _places(tensors) -> list:
+    """Where tensors of known shapes and types lie: all that a struct holds of them."""
+    return [None if x is None else (x.data_ptr(), x.stride()) for x in tensors]
 
 
 class _PolicyLoss(torch.autograd.Function):
@@ -283,9 +284,9 @@ class _PolicyLoss(torch.autograd.Function):
         saved = (logits, targets, target_index, target_prob, mask, mask_index, weights, stats)
         ctx.save_for_backward(*saved)
         ctx.status = status
-        # for a backward pass over the same storage (saved-tensor hooks may bring another): the struct, and what it
-        # points to that is a copy (the rest is held by the saved tensors alone, and freed with them)
-        ctx.packed = (_addresses(saved), None if z is logits else z, t, keep)
+        # for a backward pass over the same storage (saved-tensor hooks may bring another, or another layout of it): the
+        # struct, and what it points to that is a copy (the rest is held by the saved tensors alone, and freed with them)
+        ctx.packed = (_places(saved), None if z is logits else z, t, keep)
         return loss
 
     @staticmethod
@@ -293,8 +294,8 @@ class _PolicyLoss(torch.autograd.Function):
     def backward(ctx, upstream):
         saved = ctx.saved_tensors
         stats = saved[7]
-        addresses, z, t, keep = ctx.packed
-        if _addresses(saved) != addresses:
+        places, z, t, keep = ctx.packed
+        if _places(saved) != places:
             z, keep = _rows(saved[0], "logits"), []
             t = _targets(z, *saved[1:7], keep)
         elif z is None:

@@ -165,3 +165,34 @@ def test_loss_both_forms_give_the_same_bits(rows, vocab, dtype):
     again = lg.policy_loss(x, **kw)
     again.sum().backward()
     assert torch.equal(loss, again) and torch.equal(grad, x.grad)
+
+
+# ---- saved tensors ------------------------------------------------------------------
+def test_loss_of_tensors_that_hooks_pack_together():
+    """Hooks that bring the saved tensors back without their padding, at the same addresses."""
+    g = gen(19)
+    R, V, K, pad = 16, 700, 9, 5
+    x = torch.randn(R, V, generator=g)
+
+    def padded(t):
+        buf = torch.zeros(R, t.shape[1] + pad, dtype=t.dtype, device=DEV)
+        buf[:, :t.shape[1]] = dev(t)
+        return buf[:, :t.shape[1]]
+
+    def close_up(t):
+        if t.dim() != 2:
+            return t
+        kept = t.clone()
+        u = t.as_strided(t.shape, (t.shape[1], 1))
+        u.copy_(kept)
+        return u
+
+    for kw in (dict(targets=torch.rand(R, V, generator=g)),
+               dict(target_index=torch.randint(0, V, (R, K), generator=g), target_prob=torch.rand(R, K, generator=g))):
+        kw["mask"] = lg.pack_mask(torch.rand(R, V, generator=g) < 0.5)
+        want, grad, bl, bg = ref.loss(x, **kw)
+        leaf = dev(x).requires_grad_(True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), close_up):
+            loss = lg.policy_loss(leaf, **{k: padded(t) for k, t in kw.items()})
+        ref.close(loss, want, bl)
+        ref.close(torch.autograd.grad(loss.sum(), leaf)[0], grad, bg)
