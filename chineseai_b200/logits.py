@@ -269,37 +269,41 @@ def _places(tensors) -> list:
     return [None if x is None else (x.data_ptr(), x.stride()) for x in tensors]
 
 
+def _as_read(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """x with its last dimension contiguous, as the kernels read it."""
+    return x if x is None or x.dim() == 0 or x.stride(-1) == 1 or x.size(-1) <= 1 else x.contiguous()
+
+
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, target_index, target_prob, mask, mask_index, weights, status):
         z = _rows(logits, "logits")
-        keep: list = []
-        t = _targets(z, targets, target_index, target_prob, mask, mask_index, weights, keep)
+        inputs = [_as_read(x) for x in (targets, target_index, target_prob, mask, mask_index, weights)]
+        t = _targets(z, *inputs, [])
         n, vocab = z.shape
         dev = z.get_device()
         loss = z.new_empty(n, dtype=torch.float32)
         stats = z.new_empty(3 * n, dtype=torch.float32)
         _call("cnnue_policy_loss_fwd", dev, status, z.data_ptr(), z.stride(0), _TYPES[z.dtype], n, vocab, t,
               loss.data_ptr(), stats.data_ptr())
-        saved = (logits, targets, target_index, target_prob, mask, mask_index, weights, stats)
+        # copies that were made are saved in the place of what they are copies of, and freed with the graph
+        saved = (z, *inputs, stats)
         ctx.save_for_backward(*saved)
         ctx.status = status
-        # for a backward pass over the same storage (saved-tensor hooks may bring another, or another layout of it): the
-        # struct, and what it points to that is a copy (the rest is held by the saved tensors alone, and freed with them)
-        ctx.packed = (_places(saved), None if z is logits else z, t, keep)
+        # the struct, for a backward pass over the same storage (saved-tensor hooks may bring another, or another layout)
+        ctx.packed = _places(saved), t
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, upstream):
         saved = ctx.saved_tensors
-        stats = saved[7]
-        places, z, t, keep = ctx.packed
+        z, stats = saved[0], saved[7]
+        places, t = ctx.packed
+        keep: list = []
         if _places(saved) != places:
-            z, keep = _rows(saved[0], "logits"), []
+            z = _rows(z, "logits")
             t = _targets(z, *saved[1:7], keep)
-        elif z is None:
-            z = saved[0]
         n, vocab = z.shape
         up = upstream if upstream.dtype is torch.float32 and upstream.is_contiguous() else upstream.float().contiguous()
         grad = torch.empty_like(z)

@@ -196,3 +196,23 @@ def test_loss_of_tensors_that_hooks_pack_together():
             loss = lg.policy_loss(leaf, **{k: padded(t) for k, t in kw.items()})
         ref.close(loss, want, bl)
         ref.close(torch.autograd.grad(loss.sum(), leaf)[0], grad, bg)
+
+
+def test_loss_keeps_no_copy_after_the_backward_pass():
+    """Copies of strided logits, targets and masks are freed with the graph, though the loss lives on."""
+    g = gen(20)
+    R, V = 16, 200_000
+    x, t = (torch.randn(V, R, generator=g).to(DEV).t() for _ in range(2))
+    m = lg.pack_mask(torch.rand(R, V, generator=g) < 0.5).t().contiguous().to(DEV).t()
+    x.requires_grad_(True)
+    before = torch.cuda.memory_allocated()
+    loss = lg.policy_loss(x, t, mask=m)
+    grad, = torch.autograd.grad(loss.sum(), x)
+    want = lg.policy_loss_grad(x.detach(), t, mask=m)
+    assert torch.equal(loss, want[0]) and torch.equal(grad, want[1])
+    del grad, want
+    assert torch.cuda.memory_allocated() - before < R * V  # a quarter of one copy's bytes
+    first = lg.policy_loss(x, t, mask=m)
+    a, = torch.autograd.grad(first.sum(), x, retain_graph=True)
+    b, = torch.autograd.grad(first.sum(), x)
+    assert torch.equal(a, b)
