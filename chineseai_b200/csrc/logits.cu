@@ -491,7 +491,8 @@ int64_t row_vectors(const void* p, int64_t stride, int64_t vocab) {
 template <typename TI, typename TO>
 int pick_process(ProcArgs& a, int64_t n_rows, cudaStream_t s) {
   const int64_t nv = row_vectors<TI>(a.in, a.in_stride, a.vocab);
-  if (!a.r.history || a.r.history_len == 0 || (!a.r.repetition && !a.r.frequency && !a.r.presence)) {
+  // a history without penalties changes nothing, but its tokens and lengths are checked all the same
+  if (!a.r.history || (a.r.history_len == 0 && !a.r.lengths)) {
     a.r.history = nullptr;
     a.r.history_len = 0;
   }

@@ -216,3 +216,45 @@ def test_loss_keeps_no_copy_after_the_backward_pass():
     a, = torch.autograd.grad(first.sum(), x, retain_graph=True)
     b, = torch.autograd.grad(first.sum(), x)
     assert torch.equal(a, b)
+
+
+# ---- a history without penalties ------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab,length", [(50, 30), (2086, 200), (40_000, 100), (40_000, 5000), (40_000, 40_000)])
+def test_process_checks_a_history_without_penalties(vocab, length, dtype):
+    """Bad tokens and lengths are reported as with penalties, and nothing but the mask changes the rows."""
+    g = gen(vocab + length)
+    R = 3
+    x = (torch.randn(R, vocab, generator=g) * 3).to(dtype)
+    x[0, :3] = torch.tensor([math.inf, -math.inf, -0.0]).to(dtype)
+    h = torch.randint(-1, vocab, (R, length), generator=g)
+    h[:, :3] = torch.arange(3)
+    m = lg.pack_mask(torch.rand(R, vocab, generator=g) < 0.8)
+    want, bound = ref.process(x, mask=m)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+
+    def run(history, lengths, **kw):
+        status.zero_()
+        out = lg.process_logits(dev(x), history=dev(history), lengths=dev(lengths), status=status, **kw)
+        return out, int(status)
+
+    out, word = run(h, None, mask=dev(m))
+    ref.close(out, want, bound, dtype)
+    assert word == 0
+    bits = {torch.float32: torch.int32}.get(dtype, torch.int16)
+    out, word = run(h, None)
+    assert torch.equal(out.cpu().view(bits), x.view(bits)) and word == 0
+    bad = h.clone()
+    bad[1, length - 1] = vocab
+    out, word = run(bad, None)
+    assert torch.equal(out.cpu().view(bits), x.view(bits)) and word == 1
+    out, word = run(bad, torch.tensor([length, length - 1, length], dtype=torch.int32))  # the bad token does not count
+    assert torch.equal(out.cpu().view(bits), x.view(bits)) and word == 0
+    out, word = run(h, torch.tensor([0, length + 1, -1], dtype=torch.int32))
+    assert torch.equal(out.cpu().view(bits), x.view(bits)) and word == 2
+    out, word = run(h[:, :0], torch.tensor([0, 1, 0], dtype=torch.int32))
+    assert torch.equal(out.cpu().view(bits), x.view(bits)) and word == 2
+    y = dev(x).clone()
+    status.zero_()
+    lg.process_logits(y, history=dev(bad), out=y, status=status)  # in place, without a mask
+    assert torch.equal(y.cpu().view(bits), x.view(bits)) and int(status) == 1
