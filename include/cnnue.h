@@ -570,7 +570,7 @@ typedef struct cnnue_adamw_state {
   int64_t step;        /* steps taken; 0 before the first */
   float scalars[9];    /* written by the device: this step's fp32 factors */
   float pad[3];        /* pad[0]: 1 when the last device step was skipped;
-                          pad[1]: sqrt(1/(1-b2^t)) of the last step taken */
+                          pad[1]: sqrt(1/(1-b2^t)) of the last 8-bit step taken */
 } cnnue_adamw_state;
 int cnnue_adamw_device(float* d_params, float* d_m, float* d_v, const float* d_grads, int64_t n,
                        cnnue_adamw_state* d_state, void* stream);
