@@ -364,9 +364,10 @@ class AzTrainer:
     rank skips AdamW and raises on every rank.
 
     state_bits=8 keeps AdamW's moments in 8 bits (optim.MultiAdamW over the
-    leaves: 2.03 instead of 8 bytes per parameter); the update then runs after
-    the step's gradients instead of beside them, and a batch with a kernel
-    status changes nothing."""
+    leaves, the second moment rounded stochastically: 2.03 instead of 8 bytes
+    per parameter, sqrt(v) stays within about a factor of 2, its error's
+    standard deviation a fifth); the update then runs after the step's gradients instead of beside them, and
+    a batch with a kernel status changes nothing."""
 
     def __init__(self, weights: "az.AzWeights", lr: float = 1e-3, device: int = 0, weight_decay: float = 1e-4,
                  beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8, graph: bool = False, group=None,
@@ -418,7 +419,7 @@ class AzTrainer:
             leaves = [slice(off, min(off + n, self.n_params)) for *_, off, n in layout]
             self.optimizer = MultiAdamW([self.flat[leaf] for leaf in leaves], [self.grad[leaf] for leaf in leaves], lr=lr,
                                         beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay, state_bits=8,
-                                        device_state=True)
+                                        device_state=True, stochastic=True)
         else:
             self.m = torch.zeros(self.n_params, dtype=torch.float32, device=self.device)
             self.v = torch.zeros_like(self.m)

@@ -600,11 +600,23 @@ int cnnue_adamw_device_scaled(float* d_params, float* d_m, float* d_v, const flo
  * fp32's largest value); the update uses m' and u' before they are rounded to 8
  * bits.  A NaN or infinity in a block's m' (u') makes the scale and the codes of that
  * block's m (u) non-finite.
+ * Rounded to nearest, u hardly follows the gradients once it has settled: with
+ * b2 = 0.999 a step moves sqrt(v) by 0.05 % at most, half a step of e4m3 is 3 to
+ * 6 %, so the code comes back and only the block's scale moves.  Measured after
+ * 6,000 steps of normal gradients: u / sqrt(v) between 0.64 and 1.62 (1 % and
+ * 99 %) where nothing changes; 7.6 in the median, so steps that much too short,
+ * for elements whose gradients fell tenfold after step 1,000 while half of
+ * their block's did not.  state_bits 8 | CNNUE_ADAMW_STOCHASTIC rounds u' up
+ * with the probability that the remainder says (medians 0.98 and 1.02 there,
+ * 0.65 to 1.9), by a hash of the step, the tensor's place in the list and the
+ * element: the same call gives the same codes, on any rank.  Training of more
+ * than some hundred steps should use it.
  * copy (optional): the updated parameter rounded to copy_type (bf16 or fp16),
  * e.g. the 16-bit weights of the next forward.  Tensors of n = 0 are allowed;
  * no two tensors may overlap. */
 #define CNNUE_ADAMW_BLOCK 256
 #define CNNUE_ADAMW_NO_DECAY 1 /* flags: no weight decay for this tensor */
+#define CNNUE_ADAMW_STOCHASTIC 256 /* with state_bits 8: stochastic rounding of u' */
 typedef struct cnnue_adamw_tensor {
   void* param;
   const void* grad;
