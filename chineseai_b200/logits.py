@@ -25,6 +25,9 @@ import torch
 from ._lib import check, lib
 from .quantized import _device_stream
 
+# What a kernel wrote into a caller's tensor, told to autograd: a graph that saved it refuses its backward pass.
+_written = torch.autograd.graph.increment_version
+
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -178,6 +181,7 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     n, vocab = z.shape
     dev = z.get_device()
     code = _TYPES[z.dtype]
+    given = out
     if out is None:
         if out_dtype is None or out_dtype is z.dtype:
             out, out_code = torch.empty_like(z), code
@@ -221,6 +225,8 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     rules = _RULES.pack(*part, *bias, *_mask(mask, mask_index, n, vocab, dev, keep))
     _call("cnnue_logits_process", dev, status, z.data_ptr(), z.stride(0), code, out.data_ptr(), out.stride(0), out_code, n,
           vocab, rules)
+    if given is not None:
+        _written(given)
     return out
 
 
@@ -348,6 +354,7 @@ def policy_loss_grad(logits: torch.Tensor, targets: Optional[torch.Tensor] = Non
     t = _targets(z, targets, target_index, target_prob, mask, mask_index, weights, keep)
     n, vocab = z.shape
     dev = z.get_device()
+    given = grad
     if grad is None:
         grad = torch.empty_like(z)
     else:
@@ -360,4 +367,6 @@ def policy_loss_grad(logits: torch.Tensor, targets: Optional[torch.Tensor] = Non
     loss = z.new_empty(n, dtype=torch.float32)
     _call("cnnue_policy_loss_grad", dev, status, z.data_ptr(), z.stride(0), _TYPES[z.dtype], n, vocab, t, loss.data_ptr(),
           grad.data_ptr(), grad.stride(0))
+    if given is not None:
+        _written(given)
     return loss, grad

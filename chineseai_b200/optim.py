@@ -100,6 +100,7 @@ class MultiAdamW:
         if no_decay is not None:
             self._table["flags"] = [NO_DECAY if d else 0 for d in no_decay]
         self._check_written()
+        self._changed = self.params + [c for c in copies if c is not None]
         self._dstate = None
         if device_state:
             host = np.zeros(12, np.float64)
@@ -214,8 +215,11 @@ class MultiAdamW:
             check(lib().cnnue_adamw_multi_device(self._address, len(self.params), self._bits,
                                                  self._dstate.data_ptr(), grad_scale, *flags, stream),
                   "cnnue_adamw_multi_device")
+            torch.autograd.graph.increment_version(self._changed)
             return
         check(lib().cnnue_adamw_multi(self._address, len(self.params), self._bits, self.lr, self.beta1,
                                       self.beta2, self.eps, self.weight_decay, self._step + 1, grad_scale, *flags,
                                       stream), "cnnue_adamw_multi")
         self._step += 1
+        # told to autograd, as in-place operations are: a graph that saved a parameter refuses its backward pass
+        torch.autograd.graph.increment_version(self._changed)
