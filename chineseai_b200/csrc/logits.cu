@@ -1168,12 +1168,17 @@ int check_mask(const uint32_t* mask, int64_t stride, int64_t mask_rows, const in
   return CNNUE_OK;
 }
 
-// Whether [p, ...) and [q, ...) of the two row sets share a byte.
+// Whether the two row sets share a byte.  Rows at the same distance may lie
+// between each other's, as two column ranges of one matrix do.
 bool overlap(const void* p, int64_t p_stride, int pb, const void* q, int64_t q_stride, int qb, int64_t n_rows,
              int64_t vocab) {
   const uintptr_t p0 = (uintptr_t)p, p1 = p0 + ((n_rows - 1) * p_stride + vocab) * pb;
   const uintptr_t q0 = (uintptr_t)q, q1 = q0 + ((n_rows - 1) * q_stride + vocab) * qb;
-  return p0 < q1 && q0 < p1;
+  if (p1 <= q0 || q1 <= p0) return false;
+  const int64_t step = p_stride * pb;
+  if (n_rows == 1 || step == 0 || step != q_stride * qb || vocab * pb > step) return true;
+  const int64_t apart = ((int64_t)(q0 - p0) % step + step) % step;  // from a row of p to the next row of q
+  return apart < vocab * pb || apart + vocab * qb > step;
 }
 
 int check_targets(const cnnue_loss_targets* t, int64_t n_rows, int64_t vocab) {

@@ -9,6 +9,7 @@ import torch
 from tests import _logitsref as ref
 from tests.test_gpu_logits import DEV, TYPES, check_all, dev, gen
 from chineseai_b200 import logits as lg
+from chineseai_b200._lib import CnnueError
 
 pytestmark = pytest.mark.gpu
 
@@ -258,3 +259,38 @@ def test_process_checks_a_history_without_penalties(vocab, length, dtype):
     status.zero_()
     lg.process_logits(y, history=dev(bad), out=y, status=status)  # in place, without a mask
     assert torch.equal(y.cpu().view(bits), x.view(bits)) and int(status) == 1
+
+
+# ---- rows between each other -----------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("gap", [0, 3])
+@pytest.mark.parametrize("first", ["in", "out"])
+def test_column_ranges_of_one_matrix(first, gap, dtype):
+    """Logits and results in one matrix, side by side, as the operators' inputs and outputs; one column nearer is refused."""
+    g = gen(41)
+    R, V = 9, 333
+    x = (torch.randn(R, V, generator=g) * 3).to(dtype)
+    m = lg.pack_mask(torch.rand(R, V, generator=g) < 0.5)
+    label = torch.randint(0, V, (R,), generator=g)
+    buf = torch.full((R, 2 * V + gap + 2), 7.0, dtype=dtype, device=DEV)
+    a, b = buf[:, 1:1 + V], buf[:, 1 + V + gap:1 + 2 * V + gap]
+    z, out = (a, b) if first == "in" else (b, a)
+    z.copy_(x)
+    before = buf.clone()
+    want, bound = ref.process(x, mask=m)
+    lg.process_logits(z, mask=dev(m), out=out)
+    ref.close(out, want, bound, dtype)
+    loss, grad, bl, bg = ref.loss(x, target_index=label, mask=m)
+    got, _ = lg.policy_loss_grad(z, target_index=dev(label), mask=dev(m), grad=out)
+    ref.close(got, loss, bl)
+    ref.close(out, grad, bg, dtype)
+    out.copy_(before[:, 1 + V + gap:1 + 2 * V + gap] if first == "in" else before[:, 1:1 + V])
+    assert torch.equal(buf, before), "wrote outside the columns"
+    near = buf[:, V:2 * V] if first == "in" else buf[:, 2 + gap:2 + gap + V]
+    with pytest.raises(CnnueError, match="overlaps"):
+        lg.process_logits(z, out=near)
+    with pytest.raises(CnnueError, match="overlaps"):
+        lg.policy_loss_grad(z, target_index=dev(label), grad=near)
+    t = torch.empty(R, V + 1, dtype=dtype, device=DEV)  # rows at another distance over the same memory
+    with pytest.raises(CnnueError, match="overlaps"):
+        lg.process_logits(t[:, :V], out=t.view(-1)[:R * V].view(R, V))
