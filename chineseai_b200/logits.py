@@ -10,8 +10,11 @@ role of the policy part of compute_batch_loss
 (src/az/train_gpu_candle.rs:221-305) for whole rows of logits.
 
 All tensors are CUDA tensors on one device; calls run on that device's current
-stream, allocate only their results and can be captured in a CUDA graph when
-`status` is given.
+stream, allocate only their results (and contiguous copies of inputs whose last
+dimension is strided) and can be captured in a CUDA graph when `status` is
+given.  While policy_loss's backward pass is captured, no eager graph of the
+same leaf may live: torch ends the capture with an error then, as for its own
+operations.
 """
 from __future__ import annotations
 

@@ -294,3 +294,48 @@ def test_column_ranges_of_one_matrix(first, gap, dtype):
     t = torch.empty(R, V + 1, dtype=dtype, device=DEV)  # rows at another distance over the same memory
     with pytest.raises(CnnueError, match="overlaps"):
         lg.process_logits(t[:, :V], out=t.view(-1)[:R * V].view(R, V))
+
+
+# ---- captured calls at the sizes that take more shared memory ---------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [2086, 131_072, 250_001])
+def test_loss_forward_and_backward_captured(vocab, dtype):
+    """policy_loss with its gradient and policy_loss_grad in one graph, replayed on new logits."""
+    g = gen(vocab + 5)
+    R = 3
+    x = torch.randn(2, R, vocab, generator=g).to(dtype)
+    label = torch.randint(0, vocab, (R,), generator=g)
+    m = lg.pack_mask(torch.rand(R, vocab, generator=g) < 0.9)
+    kw = dict(target_index=dev(label), mask=dev(m), status=torch.zeros(1, dtype=torch.int32, device=DEV))
+    leaf = dev(x[0]).clone().requires_grad_(True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = lg.policy_loss(leaf, **kw)
+        grad, = torch.autograd.grad(loss.sum(), leaf)
+        fused = lg.policy_loss_grad(leaf.detach(), **kw)
+    with torch.no_grad():
+        leaf.copy_(x[1])
+    graph.replay()
+    want, gr, bl, bg = ref.loss(x[1], target_index=label, mask=m)
+    for a, b in ((loss, grad), fused):
+        ref.close(a, want, bl)
+        ref.close(b, gr, bg, dtype)
+    assert int(kw["status"]) == 0
+
+
+@pytest.mark.parametrize("vocab,length", [(16_384, 40_000), (131_072, 5000), (131_072, 40_000)])
+def test_process_captured_with_many_counters(vocab, length):
+    g = gen(length)
+    x = torch.randn(2, vocab, generator=g)
+    h = torch.randint(0, vocab, (2, length), generator=g).int()
+    f, a, hist = torch.rand(2, generator=g), dev(x).clone(), dev(h)
+    status, fd = torch.zeros(1, dtype=torch.int32, device=DEV), dev(f)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = lg.process_logits(a, history=hist, frequency=fd, status=status)
+    hist.copy_(dev(h.flip(0)))
+    graph.replay()
+    want, bound = ref.process(x, history=h.flip(0), frequency=f)
+    ref.close(out, want, bound)
+    assert int(status) == 0
