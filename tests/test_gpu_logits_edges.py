@@ -339,3 +339,49 @@ def test_process_captured_with_many_counters(vocab, length):
     want, bound = ref.process(x, history=h.flip(0), frequency=f)
     ref.close(out, want, bound)
     assert int(status) == 0
+
+
+# ---- the largest and the most rows -------------------------------------------------------
+def test_the_largest_vocabulary():
+    """2^30 tokens: sums of that many equal terms are exact, so losses and gradients are known."""
+    V = 1 << 30
+    x = torch.zeros(1, V, dtype=torch.bfloat16, device=DEV)
+    label = torch.tensor([V - 1], device=DEV)
+    loss, grad = lg.policy_loss_grad(x, target_index=label)
+    assert abs(float(loss) - 30 * math.log(2)) < 21 * 2.0 ** -21
+    assert float(grad[0, V - 1]) == -1.0 and float(grad[0, 0]) == 2.0 ** -30 and float(grad[0, V // 2]) == 2.0 ** -30
+    assert int((grad == 2.0 ** -30).sum()) == V - 1
+    del grad
+    x.requires_grad_(True)
+    again = lg.policy_loss(x, target_index=label)
+    assert torch.equal(again, loss)
+    grad, = torch.autograd.grad(again.sum(), x)
+    assert float(grad[0, V - 1]) == -1.0 and int((grad == 2.0 ** -30).sum()) == V - 1
+    del grad, again
+    x = x.detach()
+    for length in (3, 3000):  # hash table; counters of 2^15 CTAs
+        h = torch.full((length,), V - 1, dtype=torch.int32, device=DEV)
+        h[0], h[1] = 0, V // 2
+        mask = torch.full((1, V // 32), -1, dtype=torch.int32, device=DEV)
+        mask[0, V // 64] = 0
+        out = lg.process_logits(x, history=h, frequency=torch.full((1,), 0.5, device=DEV), mask=mask)
+        far = torch.tensor(-0.5 * (length - 2)).to(torch.bfloat16)  # rounded once
+        assert float(out[0, V - 1]) == float(far) and float(out[0, 0]) == -0.5
+        assert int((out == 0).sum()) == V - 32 - 2 and int((out == -math.inf).sum()) == 32
+        del out
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 7])
+def test_many_short_rows(vocab):
+    R = 1_000_003
+    x = torch.arange(R * vocab, device=DEV).view(R, vocab).remainder(5).float()
+    label = torch.arange(R, device=DEV).remainder(vocab)
+    loss, grad = lg.policy_loss_grad(x, target_index=label)
+    z = x.double()
+    want = torch.logsumexp(z, 1) - z.gather(1, label[:, None])[:, 0]
+    assert ((loss.double() - want).abs() <= 2.0 ** -19).all()  # logits of 0 .. 4: a few roundings of sums below 8
+    p = torch.softmax(z, 1).scatter_add(1, label[:, None], torch.full((R, 1), -1.0, device=DEV, dtype=torch.float64))
+    assert ((grad.double() - p).abs() <= 2.0 ** -19).all()
+    h = label[:, None].int()
+    out = lg.process_logits(x, history=h, frequency=torch.ones(R, device=DEV))
+    assert torch.equal(out, x.scatter_add(1, label[:, None], torch.full((R, 1), -1.0, device=DEV)))
